@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define LDS_ABI_VERSION 18
+#define LDS_ABI_VERSION 19
 
 /* ABI version of the loaded library (== LDS_ABI_VERSION). */
 int lds_abi_version(void);
@@ -69,6 +69,11 @@ const char* lds_error_string(int err);
  *     been written early or not at all, so θ and the draws must not be used.
  *     The word is the engine's EngineScalars.error (the `scalars` argument). */
 #define LDS_DEVERR_SGD_TILE_COUNTER 4u
+
+/* Element types of the entry points that take a `dtype` (ABI 19). */
+#define LDS_F32 0
+#define LDS_BF16 1
+#define LDS_F16 2
 
 /* Number of uint64 words per bitmask row for n nodes (ceil(n/64) rounded up
  * to an even count so every row starts 16-byte aligned). Host-only. */
@@ -465,6 +470,87 @@ int lds_sgd_clamp(float* theta, const float* grad, float lr, int64_t count,
 int lds_dropout(const float* x, int ldx, float* y, int ldy, int rows, int cols,
                 float keep_prob, float scale, uint64_t seed, uint32_t tag,
                 uint32_t counter, void* stream);
+
+/* Keyed dropout of a rows × cols block of elements `dtype` with a residual
+ * added in the same pass (ABI 19):
+ *   y = residual + (u(i, j) < keep_prob ? x * scale : 0)
+ * computed in fp32 and rounded once.  residual == NULL: lds_dropout, in any
+ * element type (fp32 gives lds_dropout's bits).  The mask is never stored: the
+ * same call on dy, without a residual, is the backward.  Rows may start at any
+ * element (row strides ldx, ldr, ldy in elements; no alignment is needed).
+ * keep_prob in [0, 1]; a dropped element is 0 (+ residual) whatever x holds
+ * there.  y does not overlap x or residual. */
+int lds_dropout_add(const void* x, int64_t ldx, const void* residual,
+                    int64_t ldr, void* y, int64_t ldy, int64_t rows, int cols,
+                    int dtype, float keep_prob, float scale, uint64_t seed,
+                    uint32_t tag, uint32_t counter, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Group norm with an activation and keyed dropout, channels last (ABI 19).
+ * x: `samples` × n × c elements `dtype`, channels contiguous, row stride ldx and
+ * sample stride sx (elements, any alignment); `groups` divides c.  For sample s
+ * and group g over its M = n·c/groups values:
+ *   mean = Σ x / M,  rstd = 1 / sqrt(Σ (x - mean)² / M + eps)
+ *   z = γ_c (x - mean) rstd + β_c
+ *   y = (u(s·n + i, c) < keep_prob ? act(z) * scale : 0)
+ * act: LDS_ACT_*.  weight (γ) / bias (β): c elements of type `ptype`, or NULL (1 and
+ * 0).  keep_prob >= 1: no dropout (scale is ignored).  y: contiguous; mean, rstd:
+ * samples × groups fp32, kept for the backward.  ws: lds_group_norm_ws_bytes
+ * bytes, 16-byte aligned, any contents, not shared by calls that may run at
+ * the same time.
+ * Statistics are fp32 sums about an element of their own group, combined as
+ * (count, mean, centred sum of squares); the last combination is fp64.
+ * ------------------------------------------------------------------------- */
+#define LDS_ACT_NONE 0
+#define LDS_ACT_RELU 1
+#define LDS_ACT_SILU 2
+int64_t lds_group_norm_ws_bytes(int64_t samples, int64_t n, int c, int groups,
+                                int dtype, int backward);
+int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx,
+                           int64_t samples, int64_t n, int c, int groups,
+                           int dtype, const void* weight, const void* bias,
+                           int ptype, float eps, int act, float keep_prob,
+                           float scale, uint64_t seed, uint32_t tag,
+                           uint32_t counter, void* y, float* mean, float* rstd,
+                           void* ws, void* stream);
+/* Backward: h = dy · mask · scale · act'(z) (z, the mask recomputed from x, mean, rstd
+ * and the key);  dweight_c = Σ h x̂,  dbias_c = Σ h  (fp32, c each; NULL: not
+ * wanted),  dx = rstd (γ h - mean_g(γ h) - x̂ mean_g(γ h x̂))  (contiguous; NULL:
+ * not wanted).  relu'(0) = 0.  dy: strides sdy, lddy, channels contiguous.
+ * Sums run in a fixed order: equal calls give equal bits. */
+int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy,
+                            const void* x, int64_t sx, int64_t ldx,
+                            int64_t samples, int64_t n, int c, int groups,
+                            int dtype, const void* weight, const void* bias,
+                            int ptype, int act, float keep_prob, float scale,
+                            uint64_t seed, uint32_t tag, uint32_t counter,
+                            const float* mean, const float* rstd, void* dx,
+                            float* dweight, float* dbias, void* ws,
+                            void* stream);
+
+/* ---------------------------------------------------------------------------
+ * 8-bit integer product with a scale for each row (node) of x and each row
+ * (output channel) of w (ABI 19).  lds_quantize_rows: for every row of x
+ * (rows × cols elements `dtype`, row stride ldx elements, any alignment)
+ *   scale = max|x| / 127 (fp32),  q = x / scale to the nearest, ties to even
+ * (of the exact quotient), |q| <= 127; the bytes of a row past cols up to ldq
+ * are set to 0.  A zero row, or one whose scale underflows to 0: q = 0,
+ * scale = 0.  A row that holds an infinity or a NaN: q = 0, scale = NaN, so that its
+ * products are NaN.  ldq: a multiple of 16, >= cols; q: 16-byte aligned.
+ * ------------------------------------------------------------------------- */
+int lds_quantize_rows(const void* x, int64_t ldx, int64_t rows, int cols,
+                      int dtype, signed char* q, int64_t ldq, float* scale,
+                      void* stream);
+/* y(i, j) = (Σ_k xq(i, k) wq(j, k)) · xs_i · ws_j + bias_j, the sum exact in int32
+ * (k <= 131071), the rest in fp32 in this order, rounded once to `dtype`.
+ * xq: m × k, wq: n × k, row strides ldx, ldw: multiples of 16 bytes; both
+ * 16-byte aligned; the bytes of a row past k up to the next multiple of 16
+ * are readable (their values are not used).  bias: n elements `ptype` or NULL.
+ * y: row stride ldy elements.  k = 0: y = bias. */
+int lds_int8_matmul(const signed char* xq, int64_t ldx, const float* xs,
+                    const signed char* wq, int64_t ldw, const float* ws,
+                    const void* bias, int ptype, int64_t m, int n, int k,
+                    void* y, int64_t ldy, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
  * θ pre-training (Pretrainer.train_step, src/trainers/pretrainer.py:68-81, used

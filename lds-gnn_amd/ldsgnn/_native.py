@@ -14,14 +14,17 @@ import os
 import torch  # noqa: F401  (must precede the CDLL: shared HIP runtime)
 
 LIB_PATH = os.environ.get("LDSGNN_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "libldsgnn.so")
-ABI_VERSION = 18
+ABI_VERSION = 19
+# the `dtype` / `ptype` arguments (LDS_F32, LDS_BF16, LDS_F16)
+ELEMENT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 c_int, c_int64, c_uint32, c_uint64, c_float, c_void_p = (
     ctypes.c_int, ctypes.c_int64, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float, ctypes.c_void_p)
 P = c_void_p  # device pointers travel as integers
 
 # name -> argtypes (restype is always int = hipError_t, except where noted)
-_RESTYPE_I64 = {"lds_bitmask_agg_ws_bytes", "lds_bitmask_agg_part_offset", "lds_planes_t128_elems", "lds_spmm_dense_ws_bytes"}  # byte counts
+_RESTYPE_I64 = {"lds_bitmask_agg_ws_bytes", "lds_bitmask_agg_part_offset", "lds_planes_t128_elems", "lds_spmm_dense_ws_bytes",
+                "lds_group_norm_ws_bytes"}  # byte counts
 SIGNATURES = {
     "lds_abi_version": [],
     "lds_graph_node_census": [P, P, c_int],
@@ -81,8 +84,17 @@ SIGNATURES = {
     "lds_sgd_clamp": [P, P, c_float, c_int64, P],
     "lds_pretrain_step": [P, c_int, P, c_int, c_float, P, P, c_int, ctypes.c_double, ctypes.c_double,
                           ctypes.c_double, ctypes.c_double, P, P],
+    "lds_dropout_add": [P, c_int64, P, c_int64, P, c_int64, c_int64, c_int, c_int, c_float, c_float, c_uint64,
+                        c_uint32, c_uint32, P],
     "lds_dropout": [P, c_int, P, c_int, c_int, c_int, c_float, c_float, c_uint64, c_uint32, c_uint32,
                     P],
+    "lds_group_norm_ws_bytes": [c_int64, c_int64, c_int, c_int, c_int, c_int],
+    "lds_group_norm_forward": [P, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int, P, P, c_int, c_float, c_int,
+                               c_float, c_float, c_uint64, c_uint32, c_uint32, P, P, P, P, P],
+    "lds_group_norm_backward": [P, c_int64, c_int64, P, c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int, P, P,
+                                c_int, c_int, c_float, c_float, c_uint64, c_uint32, c_uint32, P, P, P, P, P, P, P],
+    "lds_quantize_rows": [P, c_int64, c_int64, c_int, c_int, P, c_int64, P, P],
+    "lds_int8_matmul": [P, c_int64, P, P, c_int64, P, P, c_int, c_int64, c_int, c_int, P, c_int64, c_int, P],
     # fused engine (csrc/engine.hip)
     "lds_engine_scalars_size": [],
     "lds_sample_bitmask_dev": [P, c_int, c_uint64, c_uint32, P, c_uint32, P, c_int, P],

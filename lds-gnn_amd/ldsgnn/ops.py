@@ -399,39 +399,383 @@ def aggregate(z: torch.Tensor, graph: CsrGraph) -> torch.Tensor:
     return graph.spmm(z)
 
 
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """One entry point on `t`'s device, on that device's current stream (its
+    last argument), whatever the current device is."""
+    if t.device.index == torch.cuda.current_device():
+        nat.call(name, *args, nat.stream_of(t.device))
+    else:
+        with torch.cuda.device(t.device):
+            nat.call(name, *args, nat.stream_of(t.device))
+
+
+def _element_code(t: torch.Tensor, what: str) -> int:
+    nat.require_device(t, what)
+    code = nat.ELEMENT_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"ldsgnn {what}: expected float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _rows_of(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(tensor, rows, cols, row stride) of `t` as a rows × last-dimension block;
+    a copy only where its strides are no such block's."""
+    if t.dim() == 0:
+        raise ValueError(f"ldsgnn {what}: expected at least one dimension")
+    cols = t.size(-1)
+    if t.is_contiguous():
+        return t, (t.numel() // cols if cols else 0), cols, cols
+    rows = t.numel() // cols if cols else 0
+    try:
+        v = t.view(rows, cols)
+    except RuntimeError:
+        v = None
+    if v is None or (cols > 1 and v.stride(1) != 1) or (rows > 1 and v.stride(0) < cols):
+        return t.contiguous(), rows, cols, cols
+    return v, rows, cols, (v.stride(0) if rows > 1 else cols)
+
+
+def _keep_scale(p: float, key, what: str) -> Tuple[float, float]:
+    """(1 - p, 1 / (1 - p)) in fp32, as the kernels take them."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"ldsgnn {what}: p must lie in [0, 1], got {p}")
+    if p > 0.0 and key is None:
+        raise ValueError(f"ldsgnn {what}: dropout needs a key (seed, tag, counter)")
+    import numpy as np
+    keep = np.float32(1.0) - np.float32(p)
+    return float(keep), float(np.float32(1.0) / keep) if keep > 0 else 0.0
+
+
 class _KeyedDropout(Function):
+    """y = residual + mask(x).  Linear: the backward is the same mask on dy (at
+    any order), and dy itself for the residual."""
+
     @staticmethod
-    def forward(ctx, x, keep, scale, key):
+    def forward(ctx, x, residual, keep, scale, key):
         ctx.keep, ctx.scale, ctx.key = keep, scale, key
-        return _dropout_raw(x, keep, scale, key)
+        return _dropout_raw(x, keep, scale, key, residual)
 
     @staticmethod
     def backward(ctx, gy):
-        if torch.is_grad_enabled():
-            gx = _KeyedDropout.apply(gy, ctx.keep, ctx.scale, ctx.key)
-        else:
-            gx = _dropout_raw(gy, ctx.keep, ctx.scale, ctx.key)
-        return gx, None, None, None
+        gx = None
+        if ctx.needs_input_grad[0]:
+            if torch.is_grad_enabled():
+                gx = _KeyedDropout.apply(gy, None, ctx.keep, ctx.scale, ctx.key)
+            else:
+                gx = _dropout_raw(gy, ctx.keep, ctx.scale, ctx.key)
+        return gx, (gy if ctx.needs_input_grad[1] else None), None, None, None
 
 
-def _dropout_raw(x: torch.Tensor, keep: float, scale: float, key) -> torch.Tensor:
-    x = _f32c(x, "dropout")
-    rows, cols = x.shape
-    y = torch.empty((rows, cols), dtype=torch.float32, device=x.device)
-    seed, tag, counter = key
-    nat.call("lds_dropout", nat.ptr(x), x.stride(0), nat.ptr(y), cols, rows, cols, keep, scale, seed,
-             tag, counter, _stream(x))
+def _dropout_raw(x: torch.Tensor, keep: float, scale: float, key,
+                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    code = _element_code(x, "dropout")
+    xr, rows, cols, ldx = _rows_of(x, "dropout")
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rr, ldr = None, 0
+    if residual is not None:
+        rr, _, _, ldr = _rows_of(residual, "dropout residual")
+    seed, tag, counter = key if key is not None else (0, 0, 0)
+    _call_on(x, "lds_dropout_add", xr.data_ptr(), ldx, nat.ptr(rr), ldr, y.data_ptr(), cols, rows, cols, code, keep,
+             scale, seed, tag, counter)
     return y
 
 
-def keyed_dropout(x: torch.Tensor, p: float, key) -> torch.Tensor:
-    """F.dropout with a keyed mask: keep iff u(i, j) < 1 - p, scale 1/(1-p)."""
-    import numpy as np
-    keep = np.float32(1.0) - np.float32(p)
-    scale = np.float32(1.0) / keep
-    if x.requires_grad and torch.is_grad_enabled():
-        return _KeyedDropout.apply(x, float(keep), float(scale), key)
-    return _dropout_raw(x, float(keep), float(scale), key)
+def keyed_dropout(x: torch.Tensor, p: float, key, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """F.dropout with a keyed mask that is never stored, with an optional
+    residual added in the same pass (lds_dropout_add):
+        y = residual + (u(i, j) < 1 - p ? x / (1 - p) : 0)
+    x: float32, bfloat16 or float16, one or more dimensions, any strides; row i
+    counts the positions of all but the last dimension, j is the position in
+    it.  `residual`: shape, dtype and device of x (it is not broadcast).  The
+    result is rounded once.  key: (seed, tag, counter), see
+    ldsgnn.rng.Generator.dropout_key; p in [0, 1]."""
+    keep, scale = _keep_scale(p, key, "dropout")
+    _element_code(x, "dropout")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or
+                                 residual.device != x.device):
+        raise ValueError(f"ldsgnn dropout: the residual must match x ({tuple(x.shape)}, {x.dtype}, {x.device}), got "
+                         f"{tuple(residual.shape)}, {residual.dtype}, {residual.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _KeyedDropout.apply(x, residual, keep, scale, key)
+    return _dropout_raw(x, keep, scale, key, residual)
+
+
+# ---------------------------------------------------------------------------
+# group norm with an activation, channels last
+# ---------------------------------------------------------------------------
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+
+
+class _NormPlan:
+    """The constants of one group_norm_act call."""
+    __slots__ = ("groups", "act", "eps", "keep", "scale", "key")
+
+    def __init__(self, groups, act, eps, keep, scale, key):
+        self.groups, self.act, self.eps, self.keep, self.scale, self.key = groups, act, eps, keep, scale, key
+
+
+def _samples_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int]:
+    """(tensor, samples, n, sample stride, row stride) of a (..., n, C) tensor;
+    a copy only where its strides are no such block's."""
+    n, c = t.size(-2), t.size(-1)
+    samples = 1
+    for d in t.shape[:-2]:
+        samples *= d
+    if t.is_contiguous():
+        return t, samples, n, n * c, c
+    if t.numel() == 0:
+        return t.contiguous(), samples, n, n * c, c
+    try:
+        v = t.view(samples, n, c)
+    except RuntimeError:
+        v = None
+    if v is None or (c > 1 and v.stride(2) != 1) or (n > 1 and v.stride(1) < c):
+        return t.contiguous(), samples, n, n * c, c
+    return v, samples, n, v.stride(0), (v.stride(1) if n > 1 else c)
+
+
+def _norm_forward(x, weight, bias, pl: _NormPlan):
+    code = _element_code(x, "group_norm_act")
+    xr, samples, n, sx, ldx = _samples_of(x)
+    c = x.size(-1)
+    dev = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((2, samples, pl.groups), dtype=torch.float32, device=dev)
+    if x.numel() == 0:
+        return y, stats
+    pcode = 0 if weight is None and bias is None else nat.ELEMENT_CODES[(bias if weight is None else weight).dtype]
+    ws = torch.empty(nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 0), dtype=torch.uint8, device=dev)
+    seed, tag, counter = pl.key if pl.key is not None else (0, 0, 0)
+    at = stats.data_ptr()
+    _call_on(x, "lds_group_norm_forward", xr.data_ptr(), sx, ldx, samples, n, c, pl.groups, code, nat.ptr(weight),
+             nat.ptr(bias), pcode, pl.eps, pl.act, pl.keep, pl.scale, seed, tag, counter, y.data_ptr(), at,
+             at + 4 * samples * pl.groups, ws.data_ptr())
+    return y, stats
+
+
+def _norm_backward(gy, x, weight, bias, stats, pl: _NormPlan, need):
+    """(dx, dweight, dbias); `need`: which of them are wanted."""
+    code = _element_code(x, "group_norm_act")
+    c = x.size(-1)
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+    want_w, want_b = need[1] and weight is not None, need[2] and bias is not None
+    if x.numel() == 0:
+        return (dx, torch.zeros_like(weight) if want_w else None, torch.zeros_like(bias) if want_b else None)
+    dpar = torch.empty((2, c), dtype=torch.float32, device=dev) if want_w or want_b else None
+    xr, samples, n, sx, ldx = _samples_of(x)
+    gr, _, _, sg, ldg = _samples_of(gy)
+    pcode = 0 if weight is None and bias is None else nat.ELEMENT_CODES[(bias if weight is None else weight).dtype]
+    ws = torch.empty(nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 1), dtype=torch.uint8, device=dev)
+    seed, tag, counter = pl.key if pl.key is not None else (0, 0, 0)
+    at, dp = stats.data_ptr(), nat.ptr(dpar)
+    _call_on(x, "lds_group_norm_backward", gr.data_ptr(), sg, ldg, xr.data_ptr(), sx, ldx, samples, n, c, pl.groups,
+             code, nat.ptr(weight), nat.ptr(bias), pcode, pl.act, pl.keep, pl.scale, seed, tag, counter, at,
+             at + 4 * samples * pl.groups, nat.ptr(dx), dp if want_w else 0, dp + 4 * c if want_b else 0,
+             ws.data_ptr())
+    return (dx, dpar[0].to(weight.dtype) if want_w else None, dpar[1].to(bias.dtype) if want_b else None)
+
+
+def _norm_composed(x, weight, bias, mask, pl: _NormPlan):
+    """group_norm_act in elementary differentiable operations (fp32): what the
+    second derivative is taken of."""
+    c = x.size(-1)
+    v = x.float().reshape(-1, x.size(-2), pl.groups, c // pl.groups)
+    d = v - v.mean((1, 3), keepdim=True)
+    z = (d / (d.square().mean((1, 3), keepdim=True) + pl.eps).sqrt()).reshape(x.shape)
+    if weight is not None:
+        z = z * weight.float()
+    if bias is not None:
+        z = z + bias.float()
+    z = torch.relu(z) if pl.act == 1 else z * torch.sigmoid(z) if pl.act == 2 else z
+    return z if mask is None else torch.where(mask > 0, z * mask, torch.zeros_like(z))
+
+
+class _GroupNormAct(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, pl):
+        y, stats = _norm_forward(x, weight, bias, pl)
+        ctx.pl = pl
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight, bias, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad[:3]
+        if torch.is_grad_enabled():  # create_graph: the gradient is differentiated again
+            return _GroupNormActGrad.apply(gy, x, weight, bias, stats, ctx.pl, need) + (None,)
+        return _norm_backward(gy, x, weight, bias, stats, ctx.pl, need) + (None,)
+
+
+class _GroupNormActGrad(Function):
+    """The gradient as a function of (dy, x, weight, bias).  Its own gradient is
+    composed from elementary operations: only the hyper step of the autograd
+    path (a double backward through the inner steps) takes it."""
+
+    @staticmethod
+    def forward(ctx, gy, x, weight, bias, stats, pl, need):
+        ctx.pl, ctx.need = pl, need
+        ctx.save_for_backward(gy, x, weight, bias)
+        return _norm_backward(gy, x, weight, bias, stats, pl, need)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *cot):
+        pl, need = ctx.pl, ctx.need
+        inputs = [None if t is None else t.detach().requires_grad_(True) for t in ctx.saved_tensors]
+        gy, x, weight, bias = inputs
+        mask = None
+        if pl.keep < 1.0:
+            mask = _dropout_raw(torch.ones(x.shape, dtype=torch.float32, device=x.device), pl.keep, pl.scale, pl.key)
+        with torch.enable_grad():
+            y = _norm_composed(x, weight, bias, mask, pl)
+            wrt = [t for t, k in zip((x, weight, bias), need) if k and t is not None]
+            first = torch.autograd.grad(y, wrt, gy.float(), create_graph=True)
+            given = [c for c, t, k in zip(cot, (x, weight, bias), need) if k and t is not None]
+            live = [t for t in inputs if t is not None]
+            second = iter(torch.autograd.grad(first, live, given, allow_unused=True))
+        return tuple(None if t is None else next(second) for t in inputs) + (None, None, None)
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, act: str = "none", eps: float = 1e-5, p: float = 0.0,
+                   key=None) -> torch.Tensor:
+    """Group norm, an activation and keyed dropout in one operator, channels last
+    (lds_group_norm_forward / _backward):
+        y = mask · act((x - mean) / sqrt(var + eps) · weight + bias)
+    x: (..., n, C), float32, bfloat16 or float16, any strides; every leading
+    position is a sample of n nodes, normalised by itself over its nodes and
+    the C / groups channels of each group (biased variance).  weight, bias: C
+    values, float32, bfloat16 or float16 (both alike), or None.  act: "none",
+    "relu" or "silu".  p > 0: the mask of keyed_dropout(·, p, key) on the result.
+    Differentiable in x, weight and bias, twice where create_graph asks for it.
+    The result is rounded once; statistics and sums are fp32."""
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        raise ValueError(f"ldsgnn group_norm_act: unknown activation {act!r}; one of {sorted(ACTIVATIONS)}")
+    _element_code(x, "group_norm_act")
+    if x.dim() < 2:
+        raise ValueError(f"ldsgnn group_norm_act: expected (..., n, C), got {tuple(x.shape)}")
+    c = x.size(-1)
+    if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or c % groups:
+        raise ValueError(f"ldsgnn group_norm_act: {groups!r} groups do not divide {c} channels")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"ldsgnn group_norm_act: eps must be finite and not negative, got {eps}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (c,) or t.device != x.device or t.dtype not in nat.ELEMENT_CODES):
+            raise ValueError(f"ldsgnn group_norm_act: {name} must hold {c} floating values on {x.device}, got "
+                             f"{tuple(t.shape)}, {t.dtype}, {t.device}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("ldsgnn group_norm_act: weight and bias must share a dtype")
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    keep, scale = _keep_scale(p, key, "group_norm_act")
+    pl = _NormPlan(groups, code, float(eps), keep, scale, key if keep < 1.0 else None)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _GroupNormAct.apply(x, weight, bias, pl)
+    return _norm_forward(x, weight, bias, pl)[0]
+
+
+# ---------------------------------------------------------------------------
+# 8-bit integer product
+# ---------------------------------------------------------------------------
+
+INT8_MAX_K = 131071  # k·127·127 and k·128·128 stay below 2^31
+
+
+def int8_rows(q: torch.Tensor) -> torch.Tensor:
+    """`q` (rows × k, int8) in the layout the product reads: rows that start at
+    multiples of 16 bytes and may be read to the next one.  q itself where it
+    has that layout (quantize_rows writes it), else a copy: lay a layer's
+    weights out once."""
+    nat.require_device(q, "int8_rows")
+    if q.dtype != torch.int8 or q.dim() != 2:
+        raise TypeError(f"ldsgnn int8_rows: expected a 2-d int8 tensor, got {q.dim()}-d {q.dtype}")
+    m, k = q.shape
+    ld = q.stride(0)
+    wide = -(-k // 16) * 16
+    if k == 0 or m == 0 or (q.stride(1) == 1 and (ld >= k or m == 1) and ld % 16 == 0 and q.data_ptr() % 16 == 0 and
+                            q.untyped_storage().nbytes() - q.storage_offset() >= (m - 1) * ld + wide):
+        return q
+    out = torch.zeros((m, wide), dtype=torch.int8, device=q.device)[:, :k]
+    out.copy_(q)
+    return out
+
+
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of the rows of x (rows × k; float32, bfloat16 or float16):
+    scale = max|x| / 127 per row, q = x / scale to the nearest int8, ties to
+    even (lds_quantize_rows).  A zero row gives q = 0, scale = 0; a row with an
+    infinity or a NaN gives scale NaN.  For weights (out × in) the same call
+    gives a scale per output channel.  No gradient."""
+    code = _element_code(x, "quantize_rows")
+    if x.dim() != 2:
+        raise ValueError(f"ldsgnn quantize_rows: expected rows × k, got {tuple(x.shape)}")
+    xr, _, cols, ldx = _rows_of(x.detach(), "quantize_rows")
+    rows = x.size(0)
+    wide = -(-cols // 16) * 16
+    q = torch.empty((rows, wide), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _call_on(x, "lds_quantize_rows", xr.data_ptr(), ldx, rows, cols, code, q.data_ptr(), wide, scale.data_ptr())
+    return q[:, :cols], scale
+
+
+def _no_grad_only(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"ldsgnn {what}: the 8-bit product has no gradient; call it under torch.no_grad()")
+
+
+def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+                bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """y = (xq wqᵀ) · x_scale per row · w_scale per output channel + bias
+    (lds_int8_matmul): xq m × k and wq n × k int8 with their fp32 scales, as
+    quantize_rows gives them; the sum is exact, y is float32, bfloat16 or
+    float16, rounded once.  Rows that are not laid out as int8_rows lays them
+    out are copied.  No gradient."""
+    _no_grad_only("int8_matmul", x_scale, w_scale, bias)
+    if out_dtype not in nat.ELEMENT_CODES:
+        raise TypeError(f"ldsgnn int8_matmul: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    xq, wq = int8_rows(xq), int8_rows(wq)
+    (m, k), (n, kw) = xq.shape, wq.shape
+    dev = xq.device
+    if k != kw or k > INT8_MAX_K:
+        raise ValueError(f"ldsgnn int8_matmul: inner sizes {k} and {kw} must agree and not exceed {INT8_MAX_K}")
+    for name, t, size in (("x_scale", x_scale, m), ("w_scale", w_scale, n)):
+        if t.shape != (size,) or t.dtype != torch.float32 or t.device != dev:
+            raise ValueError(f"ldsgnn int8_matmul: {name} must be {size} float32 values on {dev}, got "
+                             f"{tuple(t.shape)}, {t.dtype}, {t.device}")
+    if wq.device != dev or (bias is not None and (bias.shape != (n,) or bias.device != dev or
+                                                  bias.dtype not in nat.ELEMENT_CODES)):
+        raise ValueError(f"ldsgnn int8_matmul: wq and bias ({n} floating values) must lie on {dev}")
+    x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    wide = -(-k // 16) * 16
+    _call_on(xq, "lds_int8_matmul", xq.data_ptr(), xq.stride(0) if m > 1 else wide, x_scale.data_ptr(),
+             wq.data_ptr(), wq.stride(0) if n > 1 else wide, w_scale.data_ptr(), nat.ptr(bias),
+             0 if bias is None else nat.ELEMENT_CODES[bias.dtype], m, n, k, y.data_ptr(), n,
+             nat.ELEMENT_CODES[out_dtype])
+    return y
+
+
+def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x (..., k) times an 8-bit weight: the rows of x are quantised
+    (quantize_rows) and multiplied (int8_matmul).  Result (..., n) in x's dtype
+    unless out_dtype names another.  No gradient."""
+    _no_grad_only("int8_linear", x, w_scale, bias)
+    _element_code(x, "int8_linear")
+    if x.dim() < 1:
+        raise ValueError("ldsgnn int8_linear: expected (..., k)")
+    rows = 1
+    for d in x.shape[:-1]:
+        rows *= d
+    q, scale = quantize_rows(x if x.dim() == 2 else x.reshape(rows, x.size(-1)))
+    y = int8_matmul(q, scale, wq, w_scale, bias, x.dtype if out_dtype is None else out_dtype)
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (y.size(1),))
 
 
 # ---------------------------------------------------------------------------
@@ -508,5 +852,6 @@ def philox_uniform(seed: int, tag: int, counter: int, rows: int, cols: int,
 
 __all__ = [
     "CsrGraph", "SampledGraph", "sample_graph_from_triu", "csr_graph_from_dense", "aggregate",
-    "keyed_dropout", "sgd_clamp_", "theta_grad", "theta_grad_form", "form_code", "philox_uniform", "TAG_DROP_X", "TAG_DROP_H",
+    "keyed_dropout", "group_norm_act", "ACTIVATIONS", "int8_rows", "quantize_rows", "int8_matmul", "int8_linear",
+    "INT8_MAX_K", "sgd_clamp_", "theta_grad", "theta_grad_form", "form_code", "philox_uniform", "TAG_DROP_X", "TAG_DROP_H",
 ]

@@ -1,0 +1,630 @@
+"""The block operators (ldsgnn.ops: keyed_dropout with a residual and in 16-bit
+types, group_norm_act, quantize_rows / int8_matmul / int8_linear) against plain
+implementations in 64 bits.
+
+Tolerances.  u = 2^-24 is fp32's largest relative rounding error, h(t) that of
+the output type (fp32 2^-24, bf16 2^-8, fp16 2^-11; fp16 results below its
+smallest normal number are off by up to 2^-25).  They are derived per operator
+at its test.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import philox
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+KEY = (0x1234567890ABCDEF, (3 << 24) | 5, 77)
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from ldsgnn import ops
+    return ops
+
+
+def mask64(key, rows, cols, p):
+    """(kept, 1 / (1 - p)) of a rows x cols block; the scale is the fp32 one."""
+    keep = np.float32(1.0) - np.float32(p)
+    u = philox.uniform(key[0], key[1], key[2], rows, cols)
+    scale = float(np.float32(1.0) / keep) if keep > 0 else 0.0
+    return torch.from_numpy(u < keep), scale
+
+
+def dropped64(x, key, p):
+    rows, cols = x.numel() // x.shape[-1], x.shape[-1]
+    if p == 0.0:
+        return x
+    kept, scale = mask64(key, rows, cols, p)
+    return torch.where(kept.view(x.shape), x * scale, torch.zeros_like(x))
+
+
+# ---------------------------------------------------------------------------
+# dropout
+# ---------------------------------------------------------------------------
+
+
+def plain_dropout(x, key, p, res=None):
+    """fp32 as the definition has it: x·scale, + residual, one rounding to the
+    type.  Every step is one IEEE operation, so the kernel has the same bits."""
+    y = x.float()
+    if p > 0.0:
+        kept, scale = mask64(key, x.numel() // x.shape[-1], x.shape[-1], p)
+        y = torch.where(kept.view(x.shape), y * np.float32(scale), torch.zeros_like(y))
+    if res is not None:
+        y = y + res.float()
+    return y.to(x.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1,), (7,), (1, 1), (3, 5), (4, 8), (37, 50), (2, 3, 33), (5, 1), (1025, 17),
+                                   (64, 1433), (2, 2, 3, 16)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_dropout_add_has_the_definition_bits(device, ops, dtype, shape, residual):
+    g = torch.Generator().manual_seed(sum(shape))
+    x = torch.randn(shape, generator=g).to(dtype)
+    res = torch.randn(shape, generator=g).to(dtype) if residual else None
+    for p in (0.0, 0.1, 0.5, 1.0):
+        y = ops.keyed_dropout(x.to(device), p, KEY, residual=None if res is None else res.to(device))
+        assert y.dtype == dtype and torch.equal(y.cpu(), plain_dropout(x, KEY, p, res)), p
+
+
+def test_dropout_strides_and_copies(device, ops):
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(6, 40, 70, generator=g).to(torch.bfloat16)
+    for cut in (lambda t: t[:, :, 3:36], lambda t: t[:, ::2, :], lambda t: t[1::2, 5:7, 1:2],
+                lambda t: t.transpose(1, 2), lambda t: t[:, :, ::3], lambda t: t[0, :1, :1].expand(9, 13),
+                lambda t: t[0, 0].expand(5, 70)):
+        x, r = cut(wide), cut(wide.neg())
+        y = ops.keyed_dropout(cut(wide.to(device)), 0.3, KEY, residual=cut(wide.neg().to(device)))
+        assert torch.equal(y.cpu(), plain_dropout(x.contiguous(), KEY, 0.3, r.contiguous()))
+
+
+def test_dropout_of_nan_and_infinity(device, ops):
+    """A dropped element is 0 (plus the residual) whatever x holds there."""
+    x = torch.full((8, 33), float("nan"))
+    x[::2] = float("inf")
+    res = torch.ones(8, 33)
+    y = ops.keyed_dropout(x.to(device), 0.5, KEY, residual=res.to(device)).cpu()
+    kept, _ = mask64(KEY, 8, 33, 0.5)
+    assert torch.equal(y[~kept], torch.ones_like(y[~kept]))
+    assert torch.isnan(y[1::2][kept[1::2]]).all() and torch.isinf(y[::2][kept[::2]]).all()
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0,), (2, 0, 3)])
+def test_dropout_empty(device, ops, shape):
+    x = torch.empty(shape, device=device, requires_grad=True)
+    y = ops.keyed_dropout(x, 0.5, KEY, residual=torch.empty(shape, device=device))
+    y.sum().backward()
+    assert y.shape == x.shape == x.grad.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dropout_gradients(device, ops, dtype):
+    """dx = the same mask on dy (the definition's bits), dres = dy; the second
+    order is the mask again; a broadcast residual's gradient is summed by its
+    own expansion."""
+    g = torch.Generator().manual_seed(9)
+    x, dy = (torch.randn(41, 27, generator=g).to(dtype) for _ in range(2))
+    r = torch.randn(27, generator=g).to(dtype)
+    xd, rd = x.to(device).requires_grad_(), r.to(device).requires_grad_()
+    y = ops.keyed_dropout(xd, 0.25, KEY, residual=rd.expand(41, 27))
+    gx, gr = torch.autograd.grad(y, (xd, rd), dy.to(device), create_graph=True)
+    assert torch.equal(gx.detach().cpu(), plain_dropout(dy, KEY, 0.25))
+    assert torch.allclose(gr.detach().cpu().double(), dy.double().sum(0), rtol=41 * HALF[dtype], atol=41 * HALF[dtype])
+    w = torch.randn(41, 27, generator=g).to(dtype).to(device).requires_grad_()
+    xw = xd.detach().requires_grad_()
+    y2 = ops.keyed_dropout(xw, 0.25, KEY)
+    (g1,) = torch.autograd.grad(y2, xw, w, create_graph=True)
+    (g2,) = torch.autograd.grad(g1, w, dy.to(device))
+    assert torch.equal(g2.cpu(), plain_dropout(dy, KEY, 0.25))
+
+
+# ---------------------------------------------------------------------------
+# group norm + activation
+# ---------------------------------------------------------------------------
+
+
+def norm64(x, groups, w, b, act, eps, key, p):
+    c = x.shape[-1]
+    v = x.reshape(-1, x.shape[-2], groups, c // groups)
+    d = v - v.mean((1, 3), keepdim=True)
+    r = 1.0 / (d.square().mean((1, 3), keepdim=True) + eps).sqrt()
+    z = (d * r).reshape(x.shape)
+    if w is not None:
+        z = z * w
+    if b is not None:
+        z = z + b
+    a = torch.relu(z) if act == "relu" else z * torch.sigmoid(z) if act == "silu" else z
+    return dropped64(a, key, p), z
+
+
+def norm_bounds(x64, groups, w, b, eps):
+    """Per element, how far the kernel's fp32 z may be from z in 64 bits:
+    mean is rounded once and comes from sums good to a few u of the values
+    about it, so x - mean is off by u (|mean| + 4 sd + |x - mean|) and x̂ by r
+    times that and 6 u |x̂| (rstd's own error and two roundings); the product
+    with γ and the sum with β round once more each.  Doubled for the sums."""
+    c = x64.shape[-1]
+    v = x64.reshape(-1, x64.shape[-2], groups, c // groups)
+    mu = v.mean((1, 3), keepdim=True)
+    d = v - mu
+    var = d.square().mean((1, 3), keepdim=True)
+    r = 1.0 / (var + eps).sqrt()
+    xe = (r * (mu.abs() + 4 * var.sqrt() + d.abs()) + 6 * (d * r).abs()) * U
+    wabs = 1.0 if w is None else w.abs()
+    z = (d * r).abs().reshape(x64.shape) * wabs
+    babs = 0.0 if b is None else b.abs()
+    return 2 * (xe.reshape(x64.shape) * wabs + 2 * U * (z + babs)), r, (d * r).reshape(x64.shape)
+
+
+NORM_SHAPES = [  # samples, n, groups, channels per group
+    (1, 1, 1, 1), (1, 1, 32, 8), (3, 1, 2, 3), (2, 7, 4, 5), (1, 5, 1, 2), (5, 33, 3, 16), (2, 100, 1, 700),
+    (1, 9, 2, 4096), (1, 3, 1, 2051), (4, 515, 12, 5), (1, 2708, 4, 4), (2, 600, 32, 8), (17, 2, 300, 2),
+]
+
+
+def norm_inputs(s, n, groups, cg, dtype, seed=0, offset=0.3):
+    g = torch.Generator().manual_seed(1000 * seed + 7 * n + groups + cg)
+    c = groups * cg
+    x = (torch.randn(s, n, c, generator=g) * 1.5 + offset).to(dtype)
+    w = torch.randn(c, generator=g) * 0.3 + 1.0
+    b = torch.randn(c, generator=g) * 0.3
+    dy = torch.randn(s, n, c, generator=g).to(dtype)
+    return x, w, b, dy
+
+
+@pytest.mark.parametrize("shape", NORM_SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,p", [("none", 0.0), ("relu", 0.5), ("silu", 0.0), ("silu", 0.1)])
+def test_group_norm_forward(device, ops, shape, dtype, act, p):
+    """|y - y64| <= h |y64| + scale (1.1 δz + 8 u |a|): δz the bound of
+    norm_bounds, 1.1 the steepest slope of the activations, 8 u for exp, the
+    reciprocal and the products of silu."""
+    s, n, groups, cg = shape
+    x, w, b, _ = norm_inputs(s, n, groups, cg, dtype)
+    y = ops.group_norm_act(x.to(device), groups, w.to(device), b.to(device), act=act, p=p, key=KEY).cpu()
+    ref, z = norm64(x.double(), groups, w.double(), b.double(), act, 1e-5, KEY, p)
+    dz, _, _ = norm_bounds(x.double(), groups, w.double(), b.double(), 1e-5)
+    scale = 1.0 if p == 0.0 else 1.0 / (1.0 - p)
+    tol = HALF[dtype] * ref.abs() + TINY[dtype] + scale * (1.1 * dz + 8 * U * z.abs())
+    assert y.dtype == dtype and y.shape == x.shape
+    assert ((y.double() - ref).abs() <= tol).all()
+
+
+def norm_grads64(x, groups, w, b, act, p, dy):
+    leaves = [t.double().requires_grad_() for t in (x, w, b)]
+    y, z = norm64(leaves[0], groups, leaves[1], leaves[2], act, 1e-5, KEY, p)
+    return torch.autograd.grad(y, leaves, dy.double()), z.detach()
+
+
+def grad_bounds(x, groups, w, b, act, p, dy):
+    """(dx, dγ, dβ) bounds.  h = dy·scale·act'(z): act' is off by δz (its slope is
+    at most 1/2 for silu, 0 else) and by 12 u (1 + |z|) of its own roundings,
+    so δh <= scale |dy| (δz + 12 u (1 + |z|)) =: e, with |h| <= 1.1 scale |dy|.
+    A sum of k terms in any order is within k u of the sum of their
+    magnitudes; a thread adds at most n values and a block at most 256 such
+    sums in a row, the rest is fp64: with x̂ off by δx̂ (norm_bounds / |γ|),
+      δ(Σ h x̂) <= Σ (e |x̂| + |h| δx̂) + (n + 258) u Σ |h x̂|.
+    dx = r (γ h - m1 - x̂ m2) adds the elementwise and the two means' errors and
+    4 roundings."""
+    s, n, c = x.shape
+    cg = c // groups
+    scale = 1.0 if p == 0.0 else 1.0 / (1.0 - p)
+    x64, w64, b64, g = x.double(), w.double(), b.double(), dy.double().abs() * scale
+    dz, r, xh = norm_bounds(x64, groups, w64, b64, 1e-5)
+    dxh, _, _ = norm_bounds(x64, groups, None, None, 1e-5)
+    z = (xh * w64 + b64).abs()
+    e = g * (dz + 12 * U * (1 + z)) if act == "silu" else g * 2 * U
+    h, xa = 1.1 * g, xh.abs()
+    sh = e.sum((0, 1)) + (n + 258) * U * h.sum((0, 1))
+    shx = (e * xa + h * dxh).sum((0, 1)) + (n + 258) * U * (h * xa).sum((0, 1))
+
+    def mean(t):
+        return t.reshape(s, n, groups, cg).mean((1, 3), keepdim=True).expand(s, n, groups, cg).reshape(s, n, c)
+
+    wa = w64.abs()
+    m1, m2 = mean(wa * h), mean(wa * h * xa)
+    e1 = mean(wa * e) + (n + 260) * U * m1
+    e2 = mean(wa * (e * xa + h * dxh)) + (n + 260) * U * m2
+    rr = r.expand(s, n, groups, cg).reshape(s, n, c)
+    dx = rr * (wa * e + e1 + xa * e2 + dxh * m2 + 12 * U * (wa * h + m1 + xa * m2))
+    return dx, shx + U * 4 * (h * xa).sum((0, 1)), sh + U * 4 * h.sum((0, 1))
+
+
+@pytest.mark.parametrize("shape", NORM_SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,p", [("none", 0.1), ("relu", 0.5), ("silu", 0.0), ("silu", 0.1)])
+def test_group_norm_backward(device, ops, shape, dtype, act, p):
+    s, n, groups, cg = shape
+    x, w, b, dy = norm_inputs(s, n, groups, cg, dtype, seed=1)
+    if act == "relu":
+        # relu's gradient jumps at 0: values nearer to it than z's own error
+        # would be decided by a last bit, so those nodes' channels are moved off it
+        for _ in range(20):
+            _, z = norm64(x.double(), groups, w.double(), b.double(), act, 1e-5, KEY, 0.0)
+            near = z.abs() < 1e-5
+            if not near.any():
+                break
+            x[near] = x[near] * 1.125 + 0.25
+        assert not near.any() or n * cg == 1
+        if n * cg == 1:
+            b = torch.where(b.abs() < 1e-3, torch.full_like(b, 0.5), b)
+    leaves = [t.to(device).requires_grad_() for t in (x, w, b)]
+    y = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act, p=p, key=KEY)
+    got = torch.autograd.grad(y, leaves, dy.to(device))
+    ref, _ = norm_grads64(x, groups, w, b, act, p, dy)
+    tol = grad_bounds(x, groups, w, b, act, p, dy)
+    for name, a, e, t, dt in zip(("dx", "dweight", "dbias"), got, ref, tol,
+                                 (dtype, torch.float32, torch.float32)):
+        assert a.dtype == dt, name
+        err = (a.cpu().double() - e).abs() - HALF[dt] * e.abs() - TINY[dt] - t
+        assert err.max() <= 0, (name, float(err.max()))
+
+
+def test_group_norm_gradient_by_differences(device, ops):
+    """The gradient against central differences of the kernel's own forward
+    (fp32): along a random direction d, (L(x + t d) - L(x - t d)) / 2t with t = 2^-6
+    differs from <grad, d> by the third derivative (order t² = 2.5e-4 relative)
+    and by the forward's rounding, 2 u |L| sqrt(N) / t; 1e-2 of the gradient's
+    norm times the direction's covers both."""
+    x, w, b, dy = norm_inputs(2, 50, 3, 8, torch.float32, seed=2)
+    g = torch.Generator().manual_seed(4)
+    leaves = [t.to(device).requires_grad_() for t in (x, w, b)]
+
+    def loss(*a):
+        return (ops.group_norm_act(a[0], 3, a[1], a[2], act="silu", p=0.2, key=KEY).double() *
+                dy.to(device).double()).sum()
+
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    for i, gr in enumerate(grads):
+        d = torch.randn(gr.shape, generator=g).to(device)
+        d = d / d.norm()
+        t = 2.0 ** -6
+        with torch.no_grad():
+            args = [[l.detach() + (sg * t * d if j == i else 0) for j, l in enumerate(leaves)] for sg in (1, -1)]
+            num = float(loss(*args[0]) - loss(*args[1])) / (2 * t)
+        assert abs(num - float((gr * d).sum())) <= 1e-2 * float(gr.norm()), i
+
+
+def test_group_norm_strides(device, ops):
+    """Slices, transposed samples, expanded samples and gradients with other
+    strides: the bits of the contiguous call."""
+    g = torch.Generator().manual_seed(6)
+    wide = torch.randn(4, 30, 52, generator=g).to(device)
+    for cut in (lambda t: t[:, :, 4:28], lambda t: t[:, :, 3:27], lambda t: t[:, 1::3, :24], lambda t: t[::2, :, 28:],
+                lambda t: t.transpose(0, 1)[:, :, :24], lambda t: t[:, :, ::2][..., :24],
+                lambda t: t[:1, :, :24].expand(3, 30, 24), lambda t: t[2, :, 10:34],
+                lambda t: t.view(2, 2, 30, 52)[..., :24]):
+        x = cut(wide).detach()
+        dy = cut(wide.cos())
+        out = []
+        for src, gy in ((x, dy), (x.contiguous(), dy.contiguous())):
+            leaf = src.detach().requires_grad_()
+            w = torch.linspace(0.5, 1.5, 24, device=device).requires_grad_()
+            y = ops.group_norm_act(leaf, 4, w, None, act="silu", p=0.3, key=KEY)
+            out.append((y,) + torch.autograd.grad(y, (leaf, w), gy))
+        for a, b in zip(*out):
+            assert torch.equal(a, b)
+
+
+def test_group_norm_samples_stand_alone(device, ops):
+    """A NaN or an infinity in one group of one sample reaches no other group;
+    a constant group gives act(β)."""
+    x, w, b, _ = norm_inputs(3, 40, 4, 8, torch.float32, seed=5)
+    x[0, 3, 9] = float("nan")
+    x[1, 7, 17] = float("inf")
+    x[2, :, 24:] = 2.5
+    y = ops.group_norm_act(x.to(device), 4, w.to(device), b.to(device), act="silu").cpu()
+    ref, _ = norm64(x.double(), 4, w.double(), b.double(), "silu", 1e-5, KEY, 0.0)
+    bad = torch.zeros(3, 40, 32, dtype=torch.bool)
+    bad[0, :, 8:16] = True
+    bad[1, :, 16:24] = True
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all()
+    assert torch.allclose(y[~bad].double(), ref[~bad], rtol=1e-5, atol=1e-5)
+    assert torch.allclose(y[2, :, 24:], (b * torch.sigmoid(b))[24:].expand(40, 8), rtol=1e-6, atol=1e-7)
+
+
+def test_group_norm_far_from_zero(device, ops):
+    """Mean 3000 sd, one outlier among the first values: the bound of
+    norm_bounds, whose term in |mean| is the mean's own last bit."""
+    x, w, b, _ = norm_inputs(2, 700, 2, 8, torch.float32, seed=8, offset=0.0)
+    x = x / 1.5 + 3000.0
+    x[:, 0, 0] = 9000.0
+    y = ops.group_norm_act(x.to(device), 2, w.to(device), b.to(device)).cpu()
+    ref, _ = norm64(x.double(), 2, w.double(), b.double(), "none", 1e-5, KEY, 0.0)
+    dz, _, _ = norm_bounds(x.double(), 2, w.double(), b.double(), 1e-5)
+    assert ((y.double() - ref).abs() <= U * ref.abs() + dz).all()
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (3, 0, 4), (0, 5, 4), (2, 3, 0)])
+def test_group_norm_empty(device, ops, shape):
+    x = torch.empty(shape, device=device, requires_grad=True)
+    w = torch.ones(shape[-1], device=device, requires_grad=True)
+    y = ops.group_norm_act(x, 1 if shape[-1] == 0 else 2, w, None, act="relu")
+    y.sum().backward()
+    assert y.shape == x.shape and x.grad.shape == x.shape and float(w.grad.sum()) == 0.0
+
+
+@pytest.mark.parametrize("weight,bias", [(True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("pdtype", DTYPES)
+def test_group_norm_parameter_forms(device, ops, weight, bias, pdtype):
+    x, w, b, dy = norm_inputs(2, 19, 2, 6, torch.bfloat16, seed=3)
+    w, b = (w.to(pdtype) if weight else None), (b.to(pdtype) if bias else None)
+    wd = None if w is None else w.to(device).requires_grad_()
+    bd = None if b is None else b.to(device).requires_grad_()
+    xd = x.to(device).requires_grad_()
+    y = ops.group_norm_act(xd, 2, wd, bd, act="silu")
+    got = torch.autograd.grad(y, [t for t in (xd, wd, bd) if t is not None], dy.to(device))
+    w64 = torch.ones(12).double() if w is None else w.double()
+    b64 = torch.zeros(12).double() if b is None else b.double()
+    ref, _ = norm_grads64(x, 2, w64, b64, "silu", 0.0, dy)
+    tol = grad_bounds(x, 2, w64, b64, "silu", 0.0, dy)
+    rows = [0] + ([1] if weight else []) + ([2] if bias else [])
+    for a, i in zip(got, rows):
+        assert a.dtype == (torch.bfloat16 if i == 0 else pdtype)
+        assert ((a.cpu().double() - ref[i]).abs() <= HALF[a.dtype] * (ref[i].abs() + tol[i]) + tol[i] +
+                TINY[a.dtype]).all()
+
+
+@pytest.mark.parametrize("act,p", [("none", 0.0), ("silu", 0.3), ("relu", 0.0)])
+def test_group_norm_second_order(device, ops, act, p):
+    """create_graph: the gradient's own gradient against 64-bit autograd.  It
+    is composed of fp32 operations; 2e-4 of the largest entry covers their
+    few hundred roundings (about 300 u) with the amplification of 1/sd."""
+    x, w, b, dy = norm_inputs(2, 15, 2, 4, torch.float32, seed=6)
+    g = torch.Generator().manual_seed(1)
+    cots = [torch.randn(t.shape, generator=g) for t in (x, w, b)]
+    out = []
+    for dev, dt in ((device, torch.float32), ("cpu", torch.float64)):
+        leaves = [t.to(dev, dt).requires_grad_() for t in (dy, x, w, b)]
+        if dev == "cpu":
+            y, _ = norm64(leaves[1], 2, leaves[2], leaves[3], act, 1e-5, KEY, p)
+        else:
+            y = ops.group_norm_act(leaves[1], 2, leaves[2], leaves[3], act=act, p=p, key=KEY)
+        first = torch.autograd.grad(y, leaves[1:], leaves[0], create_graph=True)
+        total = sum((f * c.to(dev, dt)).sum() for f, c in zip(first, cots))
+        out.append(torch.autograd.grad(total, leaves, allow_unused=True))
+    for a, e in zip(*out):
+        if e is None:
+            assert a is None or float(a.abs().max()) == 0.0
+            continue
+        assert (a.cpu().double() - e).abs().max() <= 2e-4 * max(1.0, float(e.abs().max()))
+
+
+def test_group_norm_equal_calls_equal_bits(device, ops):
+    x, w, b, dy = (t.to(device) for t in norm_inputs(3, 4001, 8, 16, torch.bfloat16, seed=4))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    runs = []
+    for _ in range(3):
+        y = ops.group_norm_act(*leaves[:1], 8, *leaves[1:], act="silu", p=0.2, key=KEY)
+        runs.append((y,) + torch.autograd.grad(y, leaves, dy))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+# ---------------------------------------------------------------------------
+# 8-bit product
+# ---------------------------------------------------------------------------
+
+
+def quantize64(x):
+    """The definition with the exact quotient's rounding decided in 64 bits:
+    x and scale are fp32 values, so a quotient that is not exactly a half is at
+    least 2^-32 of itself away from it, and 64 bits tell them apart."""
+    x = x.double()
+    top = x.abs().max(1).values if x.size(1) else torch.zeros(x.size(0), dtype=torch.float64)
+    scale = torch.from_numpy(top.numpy().astype(np.float32) / np.float32(127.0))
+    bad = ~torch.isfinite(top)
+    scale[bad] = float("nan")
+    s = scale.double()[:, None]
+    zero = bad[:, None] | (s == 0)
+    q = torch.where(zero, torch.zeros_like(x), torch.round(x / torch.where(zero, torch.ones_like(s), s)))
+    return q.clamp(-127, 127).to(torch.int8), scale
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 7), (5, 16), (2, 17), (64, 100), (33, 1433), (4, 4096), (2, 9001)])
+def test_quantize_rows(device, ops, dtype, rows, k):
+    g = torch.Generator().manual_seed(rows + k)
+    x = torch.randn(rows, k, generator=g).to(dtype)
+    q, s = ops.quantize_rows(x.to(device))
+    eq, es = quantize64(x)
+    assert q.shape == (rows, k) and q.stride(0) % 16 == 0
+    assert torch.equal(s.cpu(), es) and torch.equal(q.cpu(), eq)
+
+
+def test_quantize_rows_borders(device, ops):
+    """Ties, quotients one bit from a tie, zero rows, subnormal scales,
+    infinities, NaN."""
+    k = 300
+    x = torch.zeros(12, k)
+    x[0] = (torch.arange(k) - 150).float() + 0.5          # scale 1.1772...; general
+    x[1, 0] = 127.0                                        # scale 1: exact ties
+    x[1, 1:255] = torch.arange(-127, 127).float() + 0.5
+    x[2] = x[1]
+    x[2, 1:255] = torch.nextafter(x[1, 1:255], torch.full((254,), 1e9))
+    x[3] = x[1]
+    x[3, 1:255] = torch.nextafter(x[1, 1:255], torch.full((254,), -1e9))
+    x[4] = x[1] * 3.3333333                                # scale with many bits, near ties
+    x[6, :3] = torch.tensor([1e-45, -1e-45, 1e-44])        # scale underflows to 0
+    x[7, :4] = torch.tensor([2.5e-43, -1.3e-43, 1e-44, 0])  # subnormal scale
+    x[8, :4] = torch.tensor([3e-38, -1.7e-38, 1e-39, 0])
+    x[9, :2] = torch.tensor([3.4e38, -1.0e38])
+    x[10, 5] = float("inf")
+    x[11, 6] = float("nan")
+    q, s = ops.quantize_rows(x.to(device))
+    eq, es = quantize64(x)
+    assert torch.equal(s.cpu().isnan(), es.isnan()) and torch.equal(s.cpu().nan_to_num(), es.nan_to_num())
+    assert torch.equal(q.cpu(), eq)
+
+
+def ints(g, *shape):
+    return torch.randint(-127, 128, shape, generator=g, dtype=torch.int8)
+
+
+INT8_SHAPES = [  # m, n, k
+    (1, 1, 1), (1, 7, 16), (2, 3, 15), (5, 16, 17), (16, 16, 64), (17, 33, 65), (1, 1000, 4096), (3, 257, 1000),
+    (33, 31, 129), (64, 64, 256), (100, 7, 1433), (130, 300, 511), (257, 129, 128), (300, 520, 640), (513, 1030, 200),
+]
+
+
+@pytest.mark.parametrize("m,n,k", INT8_SHAPES)
+def test_int8_matmul_whole_numbers(device, ops, m, n, k):
+    """Scales 1, no bias: y is the integer sum, rounded to fp32 once."""
+    g = torch.Generator().manual_seed(m + n + k)
+    a, b = ints(g, m, k), ints(g, n, k)
+    one = torch.ones(max(m, n), device=device)
+    y = ops.int8_matmul(a.to(device), one[:m], b.to(device), one[:n])
+    assert torch.equal(y.cpu(), (a.double() @ b.double().t()).float())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 33, 70), (40, 50, 600), (129, 258, 300)])
+def test_int8_matmul_scales(device, ops, dtype, m, n, k):
+    """acc·xs·ws + b: four roundings (of acc to fp32, two products, the sum) and
+    the one to the type."""
+    g = torch.Generator().manual_seed(1)
+    a, b = ints(g, m, k), ints(g, n, k)
+    xs, ws, bias = torch.rand(m, generator=g) * 0.1, torch.rand(n, generator=g) * 0.1, torch.randn(n, generator=g)
+    for bd in (None, bias, bias.to(torch.bfloat16)):
+        y = ops.int8_matmul(a.to(device), xs.to(device), b.to(device), ws.to(device),
+                            None if bd is None else bd.to(device), out_dtype=dtype).cpu()
+        prod = (a.double() @ b.double().t()) * xs.double()[:, None] * ws.double()
+        ref = prod if bd is None else prod + bd.double()
+        tol = HALF[dtype] * ref.abs() + 2 * (3 * U * prod.abs() + U * ref.abs()) + TINY[dtype]
+        assert y.dtype == dtype and ((y.double() - ref).abs() <= tol).all()
+
+
+def test_int8_matmul_largest_sum(device, ops):
+    k = ops.INT8_MAX_K
+    a = torch.full((2, k), -128, dtype=torch.int8, device=device)
+    a[1] = 127
+    y = ops.int8_matmul(a, torch.ones(2, device=device), a, torch.ones(2, device=device))
+    ref = torch.tensor([[k * 16384.0, -k * 16256.0], [-k * 16256.0, k * 16129.0]], dtype=torch.float64)
+    assert torch.equal(y.cpu(), ref.float())
+
+
+def test_int8_matmul_layouts(device, ops):
+    """Rows with other bytes behind them, at odd addresses, transposed: what
+    lies past k is never used."""
+    g = torch.Generator().manual_seed(2)
+    m, n, k = 45, 70, 150
+    a, b = ints(g, m, k), ints(g, n, k)
+    ref = (a.double() @ b.double().t()).float()
+    one = torch.ones(100, device=device)
+
+    def wide(t, ld, at):
+        buf = torch.full((t.size(0) * ld + at + 64,), 85, dtype=torch.int8, device=device)
+        v = buf[at:at + t.size(0) * ld].view(t.size(0), ld)[:, :t.size(1)]
+        v.copy_(t.to(device))
+        return v
+
+    for va, vb in ((wide(a, 160, 0), wide(b, 176, 16)), (wide(a, 150, 0), wide(b, 160, 3)),
+                   (a.t().contiguous().to(device).t(), wide(b, 151, 1)), (wide(a, 192, 32), b.to(device))):
+        assert torch.equal(ops.int8_matmul(va, one[:m], vb, one[:n]).cpu(), ref)
+    # a row stride of a multiple of 16 whose last row ends with the storage
+    tight = torch.empty((m - 1) * 160 + k, dtype=torch.int8, device=device).as_strided((m, k), (160, 1))
+    tight.copy_(a)
+    assert ops.int8_rows(tight) is not tight
+    assert torch.equal(ops.int8_matmul(tight, one[:m], b.to(device), one[:n]).cpu(), ref)
+
+
+@pytest.mark.parametrize("m,n,k", [(0, 4, 8), (4, 0, 8), (3, 5, 0)])
+def test_int8_matmul_empty(device, ops, m, n, k):
+    q = torch.zeros((m, k), dtype=torch.int8, device=device)
+    w = torch.zeros((n, k), dtype=torch.int8, device=device)
+    bias = torch.arange(n, device=device).float()
+    y = ops.int8_matmul(q, torch.ones(m, device=device), w, torch.ones(n, device=device), bias)
+    assert y.shape == (m, n) and torch.equal(y, bias.expand(m, n))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,n", [((1, 64), 16), ((37,), 5), ((2, 9, 100), 33), ((300, 1433), 16), ((1, 4096), 260)])
+def test_int8_linear(device, ops, dtype, shape, n):
+    """The quantised operands are those of quantize64 exactly; the rest as in
+    test_int8_matmul_scales.  Rows of zeros give the bias, rows with a NaN give
+    NaN."""
+    g = torch.Generator().manual_seed(8)
+    k = shape[-1]
+    x = torch.randn(shape, generator=g).to(dtype)
+    w = torch.randn(n, k, generator=g) / k ** 0.5
+    bias = torch.randn(n, generator=g)
+    if x.dim() > 1 and x[..., 0].numel() > 2:
+        x.view(-1, k)[1] = 0
+        x.view(-1, k)[2, k // 2] = float("nan")
+    wq, ws = ops.quantize_rows(w.to(device))
+    with torch.no_grad():
+        y = ops.int8_linear(x.to(device), wq, ws, bias.to(device)).cpu()
+    q, s = quantize64(x.reshape(-1, k))
+    qw, sw = quantize64(w)
+    prod = (q.double() @ qw.double().t()) * s.double()[:, None] * sw.double()
+    ref = prod + bias.double()
+    y2 = y.view(-1, n).double()
+    assert y.shape == shape[:-1] + (n,) and y.dtype == dtype
+    assert torch.equal(torch.isnan(y2), torch.isnan(ref))
+    tol = HALF[dtype] * ref.abs() + 2 * (3 * U * prod.abs() + U * ref.abs()) + TINY[dtype]
+    assert ((y2 - ref).abs() <= tol)[~torch.isnan(ref)].all()
+
+
+# ---------------------------------------------------------------------------
+# streams, graphs
+# ---------------------------------------------------------------------------
+
+
+def _all_ops(ops, x, w, b, dy, wq, ws):
+    leaf = x.detach().requires_grad_()
+    wl, bl = w.detach().requires_grad_(), b.detach().requires_grad_()
+    y = ops.group_norm_act(leaf, 4, wl, bl, act="silu", p=0.25, key=KEY)
+    z = ops.keyed_dropout(y, 0.5, KEY, residual=leaf)
+    grads = torch.autograd.grad(z, (leaf, wl, bl), dy)
+    with torch.no_grad():
+        out = ops.int8_linear(z, wq, ws, b[:wq.size(0)])
+    return (z.detach(), out) + grads
+
+
+def _block_inputs(ops, device):
+    x, w, b, dy = (t.to(device) for t in norm_inputs(2, 333, 4, 16, torch.bfloat16, seed=12))
+    g = torch.Generator().manual_seed(3)
+    wq, ws = ops.quantize_rows(torch.randn(48, 64, generator=g).to(device))
+    return x, w, b, dy, wq, ws
+
+
+def test_side_stream_runs_the_same_bits(device, ops):
+    args = _block_inputs(ops, device)
+    ref = _all_ops(ops, *args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _all_ops(ops, *args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(ref, got))
+
+
+def test_captured_run_replays_the_eager_bits(device, ops):
+    """Forward, backward and the 8-bit product in one captured graph, replayed
+    with new inputs and eager work in between; kernel nodes only."""
+    import ldsgnn._native as nat
+    static = [t.clone() for t in _block_inputs(ops, device)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _all_ops(ops, *static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = nat.new_graph()
+    with torch.cuda.graph(graph):
+        out = _all_ops(ops, *static)
+    nat.seal_graph(graph, "block operators")
+    for i in range(4):
+        static[0].copy_(torch.randn_like(static[0].float()).mul_(1.0 + i))
+        static[3].copy_(torch.randn_like(static[3].float()))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        ref = _all_ops(ops, *static)
+        assert all(torch.equal(a, b) for a, b in zip(ref, got)), i
