@@ -26,33 +26,57 @@ __device__ __forceinline__ float quant_one(float x, float s, float inv) {
     return fminf(fmaxf(q, -127.f), 127.f);
 }
 
-// One block per row: the largest |x| (as bits, so that an infinity or a NaN is
-// the largest), then the row again.
-template <typename T, int V>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int cols,
-                                                            signed char* __restrict__ q, int64_t ldq,
+// G lanes per row (a power of two up to the block), R vectors of V values a lane
+// held in registers between the two uses of a row; a row longer than G R V is
+// read again.  The largest |x| is found on the bits, so that an infinity or a
+// NaN is the largest.
+template <typename T, int V, int G, int R>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows,
+                                                            int cols, signed char* __restrict__ q, int64_t ldq,
                                                             float* __restrict__ scale) {
     __shared__ uint32_t red[4];
-    const int64_t row = blockIdx.x;
-    const T* xr = x + row * ldx;
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const bool live = row < rows;
+    const int t = threadIdx.x % G;
+    const T* xr = x + (live ? row : 0) * ldx;
     uint32_t top = 0;
-    for (int j = threadIdx.x * V; j < cols; j += 256 * V) {
-        float f[V];
-        load_part<T, V>(xr + j, cols - j, f);
+    float v[R][V];
+    auto max_of = [&](const float (&f)[V]) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const uint32_t b = __float_as_uint(f[e]) & 0x7fffffffu;
             top = b > top ? b : top;
         }
+    };
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = (t + i * G) * V;
+        if (live && j < cols) {
+            load_part<T, V>(xr + j, cols - j, v[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[i][e] = 0.f;
+        }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
+    for (int i = 0; i < R; ++i) max_of(v[i]);
+    for (int64_t j = (int64_t)(t + R * G) * V; j < cols; j += G * V) {
+        float f[V];
+        load_part<T, V>(xr + j, cols - (int)j, f);
+        max_of(f);
+    }
+#pragma unroll
+    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) {
         const uint32_t b = __shfl_xor(top, o);
         top = b > top ? b : top;
     }
-    if (wave_lane() == 0) red[wave_id()] = top;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) top = red[i] > top ? red[i] : top;
+    if constexpr (G > 64) {
+        if (wave_lane() == 0) red[wave_id()] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = red[i] > top ? red[i] : top;
+    }
+    if (!live) return;
     const bool finite = top < 0x7f800000u;
     const float s = finite ? __uint_as_float(top) / 127.f : __uint_as_float(0x7fc00000u);
     const bool zero = !finite || s == 0.f;
@@ -61,21 +85,29 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     const float up = s < 1e-30f ? 18446744073709551616.f : 1.f;
     const float su = s * up;
     const float inv = zero ? 0.f : 1.f / su;
-    if (threadIdx.x == 0) scale[row] = s;
+    if (t == 0) scale[row] = s;
     signed char* qr = q + row * ldq;
-    for (int j = threadIdx.x * V; j < ldq; j += 256 * V) {
-        float f[V];
-        if (j < cols) {
-            load_part<T, V>(xr + j, cols - j, f);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) f[e] = 0.f;
-        }
+    auto put = [&](int64_t j, const float (&f)[V]) {
         typedef signed char cv __attribute__((ext_vector_type(V)));
         cv o;
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = zero ? (signed char)0 : (signed char)(int)quant_one(f[e] * up, su, inv);
         *reinterpret_cast<cv*>(qr + j) = o;  // ldq is a multiple of 16, V divides it
+    };
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int j = (t + i * G) * V;
+        if (j < ldq) put(j, v[i]);
+    }
+    for (int64_t j = (int64_t)(t + R * G) * V; j < ldq; j += G * V) {
+        float f[V];
+        if (j < cols) {
+            load_part<T, V>(xr + j, cols - (int)j, f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = 0.f;
+        }
+        put(j, f);
     }
 }
 
@@ -112,11 +144,12 @@ __device__ __forceinline__ void put_y(const Int8Args& a, T* __restrict__ y, int6
     y[i * a.ldy + j] = (T)((float)acc * a.xs[i] * a.ws[j] + b);
 }
 
-// A 16 MF x 16 NF tile of y per block; its four waves split k in 64-byte steps and
-// meet in LDS.
-template <typename T, int MF, int NF>
-__global__ __launch_bounds__(256) void int8_split_kernel(Int8Args a, T* __restrict__ y) {
-    __shared__ int red[4][MF * NF * 256];
+// A 16 MF x 16 NF tile of y per block; its W waves take W slices of k, four steps of
+// 64 bytes in flight, and meet in LDS.
+template <typename T, int MF, int NF, int W>
+__global__ __launch_bounds__(64 * W) void int8_split_kernel(Int8Args a, T* __restrict__ y) {
+    constexpr int kAhead = 4;
+    __shared__ int red[W][MF * NF * 256];
     const int nt = (a.n + 16 * NF - 1) / (16 * NF);
     const int64_t bm = blockIdx.x / nt;
     const int bn = (int)(blockIdx.x - bm * nt);
@@ -126,35 +159,54 @@ __global__ __launch_bounds__(256) void int8_split_kernel(Int8Args a, T* __restri
     const signed char* wr[NF];
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-        int64_t row = bm * (16 * MF) + 16 * i + r;
-        xr[i] = a.xq + (row < a.m ? row : a.m - 1) * a.ldx;
+        const int64_t row = bm * (16 * MF) + 16 * i + r;
+        xr[i] = a.xq + (row < a.m ? row : a.m - 1) * a.ldx + kc;
     }
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
-        int row = bn * (16 * NF) + 16 * j + r;
-        wr[j] = a.wq + (int64_t)(row < a.n ? row : a.n - 1) * a.ldw;
+        const int row = bn * (16 * NF) + 16 * j + r;
+        wr[j] = a.wq + (int64_t)(row < a.n ? row : a.n - 1) * a.ldw + kc;
     }
     v4i acc[MF][NF];
 #pragma unroll
     for (int i = 0; i < MF; ++i)
 #pragma unroll
         for (int j = 0; j < NF; ++j) acc[i][j] = v4i{0, 0, 0, 0};
-    for (int k0 = w * 64; k0 < a.k; k0 += 256) {
-        const int k = k0 + kc;
-        v4i xf[MF], wf[NF];
-#pragma unroll
-        for (int i = 0; i < MF; ++i) xf[i] = load_k(xr[i], k, a.k);
-#pragma unroll
-        for (int j = 0; j < NF; ++j) wf[j] = load_k(wr[j], k, a.k);
-        if (k0 + 64 > a.k) {
-#pragma unroll
-            for (int i = 0; i < MF; ++i) xf[i] = mask_k(xf[i], k, a.k);
-        }
+    auto mul = [&](const v4i (&xf)[MF], const v4i (&wf)[NF]) {
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
             for (int j = 0; j < NF; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xf[i], wf[j], acc[i][j], 0, 0, 0);
+    };
+    const int steps = (a.k + 63) / 64, per = (steps + W - 1) / W;
+    const int last = (w + 1) * per < steps ? (w + 1) * per : steps;
+    const int full = a.k / 64 < last ? a.k / 64 : last;  // steps before this hold 64 bytes of k
+    int t = w * per;
+    for (; t + kAhead <= full; t += kAhead) {
+        v4i xf[kAhead][MF], wf[kAhead][NF];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+            for (int j = 0; j < NF; ++j) wf[u][j] = *reinterpret_cast<const v4i*>(wr[j] + (t + u) * 64);
+#pragma unroll
+            for (int i = 0; i < MF; ++i) xf[u][i] = *reinterpret_cast<const v4i*>(xr[i] + (t + u) * 64);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) mul(xf[u], wf[u]);
+    }
+    if (t < last) {
+        v4i xf[kAhead][MF], wf[kAhead][NF];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int k0 = (t + u) * 64, end = t + u < last ? a.k - kc : 0;
+#pragma unroll
+            for (int j = 0; j < NF; ++j) wf[u][j] = load_k(wr[j], k0, end);
+#pragma unroll
+            for (int i = 0; i < MF; ++i) xf[u][i] = mask_k(load_k(xr[i], k0, end), k0, end);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) mul(xf[u], wf[u]);
     }
 #pragma unroll
     for (int i = 0; i < MF; ++i)
@@ -162,17 +214,240 @@ __global__ __launch_bounds__(256) void int8_split_kernel(Int8Args a, T* __restri
         for (int j = 0; j < NF; ++j)
             *reinterpret_cast<v4i*>(&red[w][((i * NF + j) * 64 + lane) * 4]) = acc[i][j];
     __syncthreads();
-    for (int t = threadIdx.x; t < MF * NF * 256; t += 256) {
-        const int f = t >> 8, l = (t >> 2) & 63, e = t & 3;
-        const int64_t row = bm * (16 * MF) + 16 * (f / NF) + (l >> 4) * 4 + e;
+    for (int e = threadIdx.x; e < MF * NF * 256; e += 64 * W) {
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) sum += red[i][e];
+        const int f = e >> 8, l = (e >> 2) & 63;
+        const int64_t row = bm * (16 * MF) + 16 * (f / NF) + (l >> 4) * 4 + (e & 3);
         const int col = bn * (16 * NF) + 16 * (f % NF) + (l & 15);
-        if (row < a.m && col < a.n) put_y<T>(a, y, row, col, (red[0][t] + red[1][t]) + (red[2][t] + red[3][t]));
+        if (row < a.m && col < a.n) put_y<T>(a, y, row, col, sum);
+    }
+}
+
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+__device__ const v4i kZeroChunk = {0, 0, 0, 0};
+
+// A BM x BN tile of y per block of WM x WN waves, k in steps of 64 bytes through a
+// ring of four LDS stages filled by direct loads three steps ahead.  The
+// matrix instruction is 32 x 32 x 32 with w as its first operand, so that a lane
+// ends with four neighbouring columns of one row of y.
+//
+// A stage holds the tile's rows of 64 bytes as four 16-byte chunks; chunk c of
+// row r sits at place c ^ (r / 4 % 4), so that the 16 lanes of a read phase, one
+// chunk of 16 rows, meet 16 different 16-byte bank groups.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* __restrict__ y) {
+    constexpr int kWaves = WM * WN, kStages = 4;
+    constexpr int kStageBytes = (BM + BN) * 64;
+    constexpr int kLoads = kStageBytes / 1024 / kWaves;  // direct loads per wave and stage
+    constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
+    static_assert(kStageBytes % (1024 * kWaves) == 0 && BM % 16 == 0, "whole loads per wave");
+    static_assert((kStages - 2) * kLoads <= 15, "the load count fits the wait");
+    __shared__ __attribute__((aligned(1024))) signed char smem[kStages * kStageBytes];
+    const int lane = wave_lane(), w = wave_id();
+    const int tm = (int)((a.m + BM - 1) / BM), tn = (a.n + BN - 1) / BN;
+    // Blocks go round the eight XCDs: each takes a run of neighbouring tiles,
+    // four tile rows at a time, whose operands stay in its L2.
+    const int total = tm * tn, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (id >= total) return;
+    const int band = id / (4 * tn), in_band = id - band * 4 * tn;
+    const int rows_in = tm - band * 4 < 4 ? tm - band * 4 : 4;
+    const int bm = band * 4 + in_band % rows_in, bn = in_band / rows_in;
+    const int64_t m0 = (int64_t)bm * BM;
+    const int n0 = bn * BN;
+
+    // this lane's source of every direct load: one chunk of one row
+    const signed char* src[kLoads];
+    int chunk[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int u = (w * kLoads + i) * 64 + lane;  // 16-byte place in the stage
+        const int r = u >> 2;
+        chunk[i] = ((u & 3) ^ ((r >> 2) & 3)) * 16;
+        if (r < BM) {
+            const int64_t row = m0 + r;
+            src[i] = a.xq + (row < a.m ? row : a.m - 1) * a.ldx + chunk[i];
+        } else {
+            const int row = n0 + r - BM;
+            src[i] = a.wq + (int64_t)(row < a.n ? row : a.n - 1) * a.ldw + chunk[i];
+        }
+    }
+    const int steps = (a.k + 63) / 64;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) signed char*)smem;
+    auto issue = [&](int t, bool tail) {
+        const uint32_t to = base + (t % kStages) * kStageBytes + w * kLoads * 1024;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const signed char* p = src[i] + t * 64;
+            if (tail && t * 64 + chunk[i] >= a.k) p = reinterpret_cast<const signed char*>(&kZeroChunk);
+            lds_dma16(p, to + i * 1024);
+        }
+    };
+    v16i acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+    const int wm = w % WM, wn = w / WM;
+    const int r32 = lane & 31, half = lane >> 5;
+    const int sw = (r32 >> 2) & 3;  // rows 32 apart share it
+    const signed char* xs_at = smem + (wm * (BM / WM) + r32) * 64;
+    const signed char* ws_at = smem + (BM + wn * (BN / WN) + r32) * 64;
+    // the operands of half a step: 32 bytes of k
+    auto fetch = [&](int t, int ks, v4i (&xf)[FM], v4i (&wf)[FN]) {
+        const int at = (t % kStages) * kStageBytes + (((ks * 2 + half) ^ sw) * 16);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) wf[j] = *reinterpret_cast<const v4i*>(ws_at + at + j * 2048);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) xf[i] = *reinterpret_cast<const v4i*>(xs_at + at + i * 2048);
+    };
+    auto mask = [&](int t, int ks, v4i (&xf)[FM]) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) xf[i] = mask_k(xf[i], t * 64 + (ks * 2 + half) * 16, a.k);
+    };
+    auto mul = [&](const v4i (&xf)[FM], const v4i (&wf)[FN]) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[j], xf[i], acc[i][j], 0, 0, 0);
+    };
+    // every wave's loads of a step have landed and its reads of the stage that
+    // is refilled next are done
+    auto meet = [&](int in_flight) {
+        asm volatile("" ::: "memory");
+        wait_vmcnt(in_flight);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    v4i x0[FM], w0[FN], x1[FM], w1[FN];
+    for (int t = 0; t < kStages - 1 && t < steps; ++t) issue(t, t == steps - 1);
+    {
+        const int later = steps - 1 < kStages - 2 ? steps - 1 : kStages - 2;
+        meet(later * kLoads);
+    }
+    if (kStages - 1 < steps) issue(kStages - 1, kStages == steps);
+    fetch(0, 0, x0, w0);
+    // Both halves of a step: the products of one half run while the operands of
+    // the next are read; the next step's arrival is awaited in between.
+    int t = 0;
+    for (; t + kStages < steps - 1; ++t) {
+        fetch(t, 1, x1, w1);
+        __builtin_amdgcn_sched_barrier(0);
+        mul(x0, w0);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0F70 | ((kStages - 2) * kLoads));  // vmcnt: steps t + 2 and t + 3 in flight
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        issue(t + kStages, false);
+        fetch(t + 1, 0, x0, w0);
+        __builtin_amdgcn_sched_barrier(0);
+        mul(x1, w1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; t < steps; ++t) {  // the last five steps: fewer in flight, the end of k masked
+        const bool tail = t == steps - 1;
+        fetch(t, 1, x1, w1);
+        if (tail) mask(t, 0, x0);
+        mul(x0, w0);
+        if (!tail) {
+            const int later = steps - 2 - t < kStages - 2 ? steps - 2 - t : kStages - 2;
+            meet(later * kLoads);
+            if (t + kStages < steps) issue(t + kStages, t + kStages == steps - 1);
+            fetch(t + 1, 0, x0, w0);
+        } else {
+            mask(t, 1, x1);
+        }
+        mul(x1, w1);
+    }
+    // Out through LDS, 32 rows of the wave's 64 columns at a time, so that a store
+    // writes whole lines: a lane leaves four columns of row r32 and takes VO
+    // neighbouring ones.  Unit u of row r (16 bytes) sits at place u ^ (r % 16).
+    static_assert(FN == 2 && kStages * kStageBytes >= kWaves * 8192, "an 8 KB region per wave");
+    constexpr int VO = 16 / (int)sizeof(T), kRowLanes = 64 / VO, kRows = 64 / kRowLanes;
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_s_barrier();  // every wave has read its last operands
+    asm volatile("" ::: "memory");
+    signed char* region = smem + w * 8192;
+    const int oc = lane % kRowLanes, orow = lane / kRowLanes;
+    const int col = n0 + wn * 64 + oc * VO;
+    float s[VO], b[VO];
+#pragma unroll
+    for (int e = 0; e < VO; ++e) {
+        const int cc = col + e < a.n ? col + e : a.n - 1;
+        s[e] = a.ws[cc];
+        b[e] = 0.f;
+    }
+    if (a.bias) {
+#pragma unroll
+        for (int e = 0; e < VO; ++e) b[e] = load_param(a.bias, a.ptype, col + e < a.n ? col + e : a.n - 1);
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int u = 8 * j + 2 * g + half;
+                *reinterpret_cast<v4i*>(region + r32 * 256 + (u ^ (r32 & 15)) * 16) =
+                    v4i{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();  // a wave's LDS operations are done in order
+#pragma unroll
+        for (int q = 0; q < 32 / kRows; ++q) {
+            const int r = q * kRows + orow;
+            const int64_t row = m0 + wm * (BM / WM) + 32 * i + r;
+            if (row < a.m && col < a.n) {
+                const float xs = a.xs[row];
+                float o[VO];
+#pragma unroll
+                for (int h = 0; h < VO / 4; ++h) {
+                    const v4i v = *reinterpret_cast<const v4i*>(region + r * 256 +
+                                                                ((oc * (VO / 4) + h) ^ (r & 15)) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * h + e] = (float)v[e] * xs * s[4 * h + e] + b[4 * h + e];
+                }
+                store_part<T, VO>(y + row * a.ldy + col, a.n - col, o);
+            }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
 }  // namespace lds
 
 using namespace lds;
+
+namespace {
+
+template <typename T, int MF, int NF, int W>
+int launch_split(const Int8Args& a, T* y, hipStream_t st) {
+    const int64_t blocks = ((a.m + 16 * MF - 1) / (16 * MF)) * ((a.n + 16 * NF - 1) / (16 * NF));
+    LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
+    hipLaunchKernelGGL((int8_split_kernel<T, MF, NF, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a, y);
+    LDS_RETURN_LAST_ERROR();
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+int launch_tile(const Int8Args& a, int64_t tiles, T* y, hipStream_t st) {
+    LDS_CHECK_ARG(tiles < (int64_t)1 << 30);
+    const unsigned blocks = (unsigned)((tiles + 7) / 8 * 8);  // whole rounds of the eight XCDs
+    hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WM, WN>), dim3(blocks), dim3(64 * WM * WN), 0, st, a, y);
+    LDS_RETURN_LAST_ERROR();
+}
+
+}  // namespace
 
 extern "C" int lds_quantize_rows(const void* x, int64_t ldx, int64_t rows, int cols, int dtype, signed char* q,
                                  int64_t ldq, float* scale, void* stream) {
@@ -183,8 +458,20 @@ extern "C" int lds_quantize_rows(const void* x, int64_t ldx, int64_t rows, int c
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
         constexpr int V = 16 / (int)sizeof(T);
-        hipLaunchKernelGGL((quantize_rows_kernel<T, V>), dim3((unsigned)rows), dim3(256), 0, (hipStream_t)stream,
-                           (const T*)x, ldx, cols, q, ldq, scale);
+        auto go = [&](auto lanes, auto regs) {
+            constexpr int G = decltype(lanes)::value, R = decltype(regs)::value;
+            hipLaunchKernelGGL((quantize_rows_kernel<T, V, G, R>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))),
+                               dim3(256), 0, (hipStream_t)stream, (const T*)x, ldx, rows, cols, q, ldq, scale);
+        };
+        // a row in the registers of 16 lanes, of a wave or of a block
+        if (ldq <= 16 * V)
+            go(IntC<16>{}, IntC<1>{});
+        else if (ldq <= 64 * V)
+            go(IntC<64>{}, IntC<1>{});
+        else if (ldq <= 64 * V * 4)
+            go(IntC<64>{}, IntC<4>{});
+        else
+            go(IntC<256>{}, IntC<4>{});
         LDS_RETURN_LAST_ERROR();
     });
 }
@@ -199,12 +486,14 @@ extern "C" int lds_int8_matmul(const signed char* xq, int64_t ldx, const float* 
     LDS_CHECK_ARG(k == 0 || (xq && wq && ldx >= k && ldw >= k && ldx % 16 == 0 && ldw % 16 == 0 &&
                              (((uintptr_t)xq | (uintptr_t)wq) & 15) == 0));
     const Int8Args a{xq, wq, xs, ws, bias, ldx, ldw, ldy, m, n, k, ptype};
-    const int64_t blocks = ((m + 31) / 32) * ((n + 31) / 32);
-    LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
+    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), mid = ((m + 127) / 128) * ((n + 127) / 128);
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
-        hipLaunchKernelGGL((int8_split_kernel<T, 2, 2>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a,
-                           (T*)y);
-        LDS_RETURN_LAST_ERROR();
+        const hipStream_t st = (hipStream_t)stream;
+        if (k > 0 && big >= 192) return launch_tile<T, 256, 256, 2, 4>(a, big, (T*)y, st);
+        if (k > 0 && mid >= 192) return launch_tile<T, 128, 128, 2, 2>(a, mid, (T*)y, st);
+        if (m <= 16) return launch_split<T, 1, 1, 8>(a, (T*)y, st);
+        if (m <= 32) return launch_split<T, 2, 1, 8>(a, (T*)y, st);
+        return launch_split<T, 2, 2, 8>(a, (T*)y, st);
     });
 }

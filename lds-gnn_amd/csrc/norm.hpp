@@ -162,10 +162,6 @@ __device__ __forceinline__ float act_grad(float z) {
 }
 
 // Calls f with an integral constant for the activation.
-template <int N>
-struct IntC {
-    static constexpr int value = N;
-};
 template <typename F>
 inline int with_act(int act, F&& f) {
     if (act == LDS_ACT_NONE) return f(IntC<LDS_ACT_NONE>{});

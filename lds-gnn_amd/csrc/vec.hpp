@@ -112,6 +112,12 @@ inline bool drop_key(float keep, float scale, uint64_t seed, uint32_t tag, uint3
     return t < 16777216.0;
 }
 
+// A compile-time int as a value.
+template <int N>
+struct IntC {
+    static constexpr int value = N;
+};
+
 // Calls f with a value of the element type.
 template <typename F>
 inline int with_type(int code, F&& f) {

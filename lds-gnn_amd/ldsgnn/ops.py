@@ -686,23 +686,43 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] 
 INT8_MAX_K = 131071  # k·127·127 and k·128·128 stay below 2^31
 
 
-def int8_rows(q: torch.Tensor) -> torch.Tensor:
-    """`q` (rows × k, int8) in the layout the product reads: rows that start at
-    multiples of 16 bytes and may be read to the next one.  q itself where it
-    has that layout (quantize_rows writes it), else a copy: lay a layer's
-    weights out once."""
-    nat.require_device(q, "int8_rows")
+def _int8_stride(k: int) -> int:
+    """Row stride (bytes) of the 8-bit layouts: an odd number of 64-byte lines, so
+    that the 16 rows a wave reads at once do not fall on the same cache sets
+    (16 x 4096 x 4096: 5.9 us at stride 4096, 4.8 at 4160); short rows are only
+    padded to 16 bytes."""
+    return -(-k // 16) * 16 if k <= 64 else (-(-k // 64) | 1) * 64
+
+
+def _int8_readable(q: torch.Tensor, what: str) -> torch.Tensor:
+    """q where the product can read it (16-byte rows that end inside their
+    storage), else a copy."""
+    nat.require_device(q, what)
     if q.dtype != torch.int8 or q.dim() != 2:
-        raise TypeError(f"ldsgnn int8_rows: expected a 2-d int8 tensor, got {q.dim()}-d {q.dtype}")
+        raise TypeError(f"ldsgnn {what}: expected a 2-d int8 tensor, got {q.dim()}-d {q.dtype}")
     m, k = q.shape
-    ld = q.stride(0)
-    wide = -(-k // 16) * 16
-    if k == 0 or m == 0 or (q.stride(1) == 1 and (ld >= k or m == 1) and ld % 16 == 0 and q.data_ptr() % 16 == 0 and
-                            q.untyped_storage().nbytes() - q.storage_offset() >= (m - 1) * ld + wide):
+    if m == 0 or k == 0:
         return q
-    out = torch.zeros((m, wide), dtype=torch.int8, device=q.device)[:, :k]
+    ld = q.stride(0) if m > 1 else 16
+    if (q.stride(1) == 1 or k == 1) and (ld >= k or m == 1) and ld % 16 == 0 and q.data_ptr() % 16 == 0 and \
+            q.untyped_storage().nbytes() - q.storage_offset() >= (m - 1) * ld + -(-k // 16) * 16:
+        return q
+    return _int8_layout(q)
+
+
+def _int8_layout(q: torch.Tensor) -> torch.Tensor:
+    out = torch.zeros((q.size(0), _int8_stride(q.size(1))), dtype=torch.int8, device=q.device)[:, :q.size(1)]
     out.copy_(q)
     return out
+
+
+def int8_rows(q: torch.Tensor) -> torch.Tensor:
+    """`q` (rows × k, int8) in the layout that the product reads best, the one
+    quantize_rows writes: lay a layer's weights out once.  q itself where it has
+    that layout; the product takes other layouts too, and copies the rows that
+    it cannot read in place."""
+    r = _int8_readable(q, "int8_rows")
+    return r if r.size(0) <= 1 or r.size(1) == 0 or r.stride(0) == _int8_stride(r.size(1)) else _int8_layout(r)
 
 
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -716,7 +736,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"ldsgnn quantize_rows: expected rows × k, got {tuple(x.shape)}")
     xr, _, cols, ldx = _rows_of(x.detach(), "quantize_rows")
     rows = x.size(0)
-    wide = -(-cols // 16) * 16
+    wide = _int8_stride(cols)
     q = torch.empty((rows, wide), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     _call_on(x, "lds_quantize_rows", xr.data_ptr(), ldx, rows, cols, code, q.data_ptr(), wide, scale.data_ptr())
@@ -733,12 +753,12 @@ def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_sca
     """y = (xq wqᵀ) · x_scale per row · w_scale per output channel + bias
     (lds_int8_matmul): xq m × k and wq n × k int8 with their fp32 scales, as
     quantize_rows gives them; the sum is exact, y is float32, bfloat16 or
-    float16, rounded once.  Rows that are not laid out as int8_rows lays them
-    out are copied.  No gradient."""
+    float16, rounded once.  Rows that do not start at multiples of 16 bytes are
+    copied (int8_rows lays them out once).  No gradient."""
     _no_grad_only("int8_matmul", x_scale, w_scale, bias)
     if out_dtype not in nat.ELEMENT_CODES:
         raise TypeError(f"ldsgnn int8_matmul: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    xq, wq = int8_rows(xq), int8_rows(wq)
+    xq, wq = _int8_readable(xq, "int8_matmul"), _int8_readable(wq, "int8_matmul")
     (m, k), (n, kw) = xq.shape, wq.shape
     dev = xq.device
     if k != kw or k > INT8_MAX_K:
@@ -754,8 +774,8 @@ def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_sca
     bias = bias if bias is None else bias.contiguous()
     y = torch.empty((m, n), dtype=out_dtype, device=dev)
     wide = -(-k // 16) * 16
-    _call_on(xq, "lds_int8_matmul", xq.data_ptr(), xq.stride(0) if m > 1 else wide, x_scale.data_ptr(),
-             wq.data_ptr(), wq.stride(0) if n > 1 else wide, w_scale.data_ptr(), nat.ptr(bias),
+    _call_on(xq, "lds_int8_matmul", xq.data_ptr(), xq.stride(0) if m > 1 and k > 0 else wide, x_scale.data_ptr(),
+             wq.data_ptr(), wq.stride(0) if n > 1 and k > 0 else wide, w_scale.data_ptr(), nat.ptr(bias),
              0 if bias is None else nat.ELEMENT_CODES[bias.dtype], m, n, k, y.data_ptr(), n,
              nat.ELEMENT_CODES[out_dtype])
     return y
