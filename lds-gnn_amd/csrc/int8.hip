@@ -237,14 +237,15 @@ __device__ const v4i kZeroChunk = {0, 0, 0, 0};
 // A stage holds the tile's rows of 64 bytes as four 16-byte chunks; chunk c of
 // row r sits at place c ^ (r / 4 % 4), so that the 16 lanes of a read phase, one
 // chunk of 16 rows, meet 16 different 16-byte bank groups.
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int kStages>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* __restrict__ y) {
-    constexpr int kWaves = WM * WN, kStages = 4;
+    constexpr int kWaves = WM * WN;
     constexpr int kStageBytes = (BM + BN) * 64;
     constexpr int kLoads = kStageBytes / 1024 / kWaves;  // direct loads per wave and stage
     constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
     static_assert(kStageBytes % (1024 * kWaves) == 0 && BM % 16 == 0, "whole loads per wave");
-    static_assert((kStages - 2) * kLoads <= 15, "the load count fits the wait");
+    constexpr int kFlight = (kStages - 2) * kLoads;  // this wave's loads that may stay in flight
+    static_assert(kFlight <= 63, "the load count fits the wait");
     __shared__ __attribute__((aligned(1024))) signed char smem[kStages * kStageBytes];
     const int lane = wave_lane(), w = wave_id();
     const int tm = (int)((a.m + BM - 1) / BM), tn = (a.n + BN - 1) / BN;
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* 
         mul(x0, w0);
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0F70 | ((kStages - 2) * kLoads));  // vmcnt: steps t + 2 and t + 3 in flight
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (kFlight & 15) | (kFlight >> 4 << 14));  // vmcnt(kFlight)
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* 
         mul(x1, w1);
         __builtin_amdgcn_sched_barrier(0);
     }
-    for (; t < steps; ++t) {  // the last five steps: fewer in flight, the end of k masked
+    for (; t < steps; ++t) {  // the last kStages + 1 steps: fewer in flight, the end of k masked
         const bool tail = t == steps - 1;
         fetch(t, 1, x1, w1);
         if (tail) mask(t, 0, x0);
@@ -439,11 +440,12 @@ int launch_split(const Int8Args& a, T* y, hipStream_t st) {
     LDS_RETURN_LAST_ERROR();
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
-int launch_tile(const Int8Args& a, int64_t tiles, T* y, hipStream_t st) {
+template <typename T, int BM, int BN, int WM, int WN, int S>
+int launch_tile(const Int8Args& a, T* y, hipStream_t st) {
+    const int64_t tiles = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
     LDS_CHECK_ARG(tiles < (int64_t)1 << 30);
     const unsigned blocks = (unsigned)((tiles + 7) / 8 * 8);  // whole rounds of the eight XCDs
-    hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WM, WN>), dim3(blocks), dim3(64 * WM * WN), 0, st, a, y);
+    hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WM, WN, S>), dim3(blocks), dim3(64 * WM * WN), 0, st, a, y);
     LDS_RETURN_LAST_ERROR();
 }
 
@@ -486,14 +488,23 @@ extern "C" int lds_int8_matmul(const signed char* xq, int64_t ldx, const float* 
     LDS_CHECK_ARG(k == 0 || (xq && wq && ldx >= k && ldw >= k && ldx % 16 == 0 && ldw % 16 == 0 &&
                              (((uintptr_t)xq | (uintptr_t)wq) & 15) == 0));
     const Int8Args a{xq, wq, xs, ws, bias, ldx, ldw, ldy, m, n, k, ptype};
-    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), mid = ((m + 127) / 128) * ((n + 127) / 128);
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
         const hipStream_t st = (hipStream_t)stream;
-        if (k > 0 && big >= 192) return launch_tile<T, 256, 256, 2, 4>(a, big, (T*)y, st);
-        if (k > 0 && mid >= 192) return launch_tile<T, 128, 128, 2, 2>(a, mid, (T*)y, st);
-        if (m <= 16) return launch_split<T, 1, 1, 8>(a, (T*)y, st);
-        if (m <= 32) return launch_split<T, 2, 1, 8>(a, (T*)y, st);
-        return launch_split<T, 2, 2, 8>(a, (T*)y, st);
+        // The largest tile that gives three quarters of the 256 CUs one each; below
+        // that (few rows, or few columns) k is split over a block's waves, with the
+        // smallest tile that stays within 384 blocks.
+        const auto tiles = [&](int bm, int bn) { return ((m + bm - 1) / bm) * (int64_t)((n + bn - 1) / bn); };
+        if (k > 0) {
+            if (tiles(256, 256) >= 192) return launch_tile<T, 256, 256, 2, 4, 4>(a, (T*)y, st);
+            if (tiles(256, 128) >= 192) return launch_tile<T, 256, 128, 4, 2, 4>(a, (T*)y, st);
+            if (tiles(128, 128) >= 192) return launch_tile<T, 128, 128, 2, 2, 4>(a, (T*)y, st);
+            if (tiles(128, 64) >= 192) return launch_tile<T, 128, 64, 4, 1, 6>(a, (T*)y, st);
+            if (tiles(64, 64) >= 192) return launch_tile<T, 64, 64, 2, 1, 4>(a, (T*)y, st);
+        }
+        if (tiles(16, 16) <= 384) return launch_split<T, 1, 1, 8>(a, (T*)y, st);
+        if (tiles(32, 16) <= 384) return launch_split<T, 2, 1, 8>(a, (T*)y, st);
+        if (tiles(32, 32) <= 384) return launch_split<T, 2, 2, 8>(a, (T*)y, st);
+        return launch_split<T, 4, 2, 8>(a, (T*)y, st);
     });
 }

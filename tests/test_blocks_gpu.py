@@ -471,7 +471,8 @@ def ints(g, *shape):
 INT8_SHAPES = [  # m, n, k
     (1, 1, 1), (1, 7, 16), (2, 3, 15), (5, 16, 17), (16, 16, 64), (17, 33, 65), (1, 1000, 4096), (3, 257, 1000),
     (33, 31, 129), (64, 64, 256), (100, 7, 1433), (130, 300, 511), (257, 129, 128), (300, 520, 640), (513, 1030, 200),
-    (3600, 3590, 200), (3585, 3600, 64), (1100, 1025, 333),
+    (3600, 3590, 200), (3585, 3600, 64), (1100, 1025, 333), (2500, 2300, 65), (1600, 2000, 129), (900, 1700, 700),
+    (777, 900, 1000), (2708, 16, 1433), (500, 120, 2049),
 ]
 
 
