@@ -59,14 +59,19 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ 
             if constexpr (RES) load_part<T, V>(res + (i0 + r) * ldr + j, w, a[r]);
         }
     }
-    const uint32_t keep = DROP ? keep_bits<V>(key, (uint32_t)j, (uint32_t)rq) : 0u;
+    bool kept[4][V];
+    if constexpr (DROP) {
+        ColumnKeep<V> columns;
+        columns.init(key, (uint32_t)j);
+        columns.quad(key, (uint32_t)rq, kept);
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if (i0 + r >= rows) break;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             float o = v[r][e];
-            if constexpr (DROP) o = (keep >> (4 * e + r)) & 1u ? o * key.scale : 0.f;
+            if constexpr (DROP) o = kept[r][e] ? o * key.scale : 0.f;
             if constexpr (RES) o = o + a[r][e];
             v[r][e] = o;
         }

@@ -4,58 +4,30 @@
 // A thread owns V neighbouring channels of one group (V divides the channels
 // per group) and walks row quads: four rows whose flat indices s·n + i differ in
 // their two low bits, the unit in which the keyed dropout mask is drawn.
+//
+// Two forms.  "Slab": a block keeps a sample's rows of a few groups in its
+// registers, so that x is read once and one launch does it all.  "Parts": a
+// sample's rows are cut into parts, whose sums are written, combined by a
+// small launch, and used by a second pass over x.
 #pragma once
 
 #include "vec.hpp"
 
 namespace lds {
 
-constexpr int kNormThreads = 256;
-
-// How the channels of a row are cut: a block takes `lanes` vectors of V
-// channels and `ty` rows at a time; `chunks` blocks cover a row.  A chunk
-// holds whole groups, or (a group wider than 256 vectors) one of the `sub`
-// parts of a group.
-struct NormCut {
-    int v, lanes, ty, chunks, lpg, sub;
-};
-
-inline NormCut norm_cut(int c, int groups, int v) {
-    NormCut k;
-    const int cg = c / groups;
-    k.v = v;
-    const int lpg = cg / v;  // vectors per group
-    if (lpg <= kNormThreads) {
-        int per = kNormThreads / lpg;
-        if (per > groups) per = groups;
-        k.chunks = (groups + per - 1) / per;
-        per = (groups + k.chunks - 1) / k.chunks;  // even chunks
-        k.chunks = (groups + per - 1) / per;
-        k.lanes = per * lpg;
-        k.lpg = lpg;
-        k.sub = 1;
-    } else {
-        k.sub = (lpg + kNormThreads - 1) / kNormThreads;
-        k.lanes = (lpg + k.sub - 1) / k.sub;
-        k.lpg = k.lanes;
-        k.chunks = groups * k.sub;
-    }
-    k.ty = kNormThreads / k.lanes;
-    return k;
-}
-
-// The widest vector (<= 16 bytes) that lies in one group: 1, 2, 4 or 8 channels.
-inline int norm_vec(int c, int groups, int elem_bytes) {
-    const int cg = c / groups;
-    for (int v = 16 / elem_bytes; v > 1; v /= 2)
-        if (cg % v == 0) return v;
-    return 1;
-}
+constexpr int kNormThreads = 256;  // a block of the parts form
+constexpr int kNormBlocks = 4096;  // blocks of a pass of the parts form: up to 16 per CU
+constexpr int kSlabQuads = 4;      // row quads that a slab thread holds at most
+constexpr int kForwardSlabThreads = 1024;
+constexpr int kBackwardSlabThreads = 512;  // x and dy: twice the registers a thread
 
 struct NormArgs {
     int64_t samples, n, sx, ldx;
     int c, groups, cg;
-    int lanes, ty, chunks, lpg, sub;
+    int lanes;        // vectors of a row that a block takes
+    int ty;           // row quads that it takes at a time
+    int chunks;       // blocks across a row
+    int lpg, sub;     // vectors per group (in the chunk); chunks per group
     int parts;        // row parts per sample
     int64_t part_q;   // row quads per part
     const void* weight;
@@ -64,85 +36,133 @@ struct NormArgs {
     DropKey key;
 };
 
-// What a thread of a block works on.
+// What a thread works on.
 struct NormPlace {
     int64_t s;            // sample
     int part, chunk;
-    int tx, row0, stride;  // vector in the chunk, first quad of the thread, quads per step
-    int group, c0;         // the thread's group and its first channel
+    int tx, ty;           // vector in the chunk, first row quad of the thread in the part
+    int group, c0;        // the thread's group and its first channel
     bool live;
-    int64_t q0, q1;        // the part's row quads (flat index / 4)
-    int64_t f0, f1;        // the sample's flat rows
+    int64_t q0, q1;       // the part's row quads (flat index / 4)
+    int64_t f0, f1;       // the sample's flat rows
 };
 
-__device__ __forceinline__ NormPlace norm_place(const NormArgs& a, int v) {
+__device__ __forceinline__ NormPlace norm_place(const NormArgs& a, int v, int64_t s, int part, int chunk) {
     NormPlace p;
-    int64_t b = blockIdx.x;
-    p.chunk = (int)(b % a.chunks);
-    b /= a.chunks;
-    p.part = (int)(b % a.parts);
-    p.s = b / a.parts;
-    const int t = threadIdx.x;
-    p.row0 = t / a.lanes;
-    p.tx = t - p.row0 * a.lanes;
-    p.stride = a.ty;
+    p.s = s;
+    p.part = part;
+    p.chunk = chunk;
+    p.ty = (int)((unsigned)threadIdx.x / (unsigned)a.lanes);
+    p.tx = (int)threadIdx.x - p.ty * a.lanes;
     if (a.sub == 1) {
         const int per = a.lanes / a.lpg;
         const int gi = p.tx / a.lpg;
-        p.group = p.chunk * per + gi;
+        p.group = chunk * per + gi;
         p.c0 = p.group * a.cg + (p.tx - gi * a.lpg) * v;
-        p.live = p.row0 < a.ty && p.group < a.groups;
+        p.live = p.ty < a.ty && p.group < a.groups;
     } else {
-        p.group = p.chunk / a.sub;
-        const int at = ((p.chunk - p.group * a.sub) * a.lanes + p.tx) * v;
+        p.group = chunk / a.sub;
+        const int at = ((chunk - p.group * a.sub) * a.lanes + p.tx) * v;
         p.c0 = p.group * a.cg + at;
-        p.live = p.row0 < a.ty && at < a.cg;
+        p.live = p.ty < a.ty && at < a.cg;
     }
-    p.f0 = p.s * a.n;
+    p.f0 = s * a.n;
     p.f1 = p.f0 + a.n;
-    p.q0 = (p.f0 >> 2) + (int64_t)p.part * a.part_q;
+    p.q0 = (p.f0 >> 2) + (int64_t)part * a.part_q;
     const int64_t qe = ((p.f1 - 1) >> 2) + 1;
     p.q1 = p.q0 + a.part_q < qe ? p.q0 + a.part_q : qe;
     return p;
 }
 
-// Merges the values of a row quad (rows with in[r]) into running moments.
-template <int V>
-__device__ __forceinline__ void quad_moments(const float (&v)[4][V], const bool (&in)[4], double& mean, float& m2,
-                                             float& cnt) {
-    float k = 0.f, m = 0.f;
-#pragma unroll
-    for (int r = 3; r >= 0; --r) {
-        k = in[r] ? v[r][0] : k;
-        m += in[r] ? (float)V : 0.f;
-    }
-    if (m == 0.f) return;
-    float d[4][V], s1 = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            d[r][e] = in[r] ? v[r][e] - k : 0.f;
-            s1 += d[r][e];
-        }
-    const float mq = s1 * __builtin_amdgcn_rcpf(m);
-    float s2 = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float t = in[r] ? d[r][e] - mq : 0.f;
-            s2 = __builtin_fmaf(t, t, s2);
-        }
-    const double delta = ((double)k + (double)mq) - mean;
-    const float part = m * __builtin_amdgcn_rcpf(cnt + m);
-    mean += delta * (double)part;
-    m2 += __builtin_fmaf((float)delta * (float)delta, cnt * part, s2);
-    cnt += m;
+__device__ __forceinline__ NormPlace norm_part_place(const NormArgs& a, int v) {
+    const unsigned b = blockIdx.x, row = b / (unsigned)a.chunks;
+    const unsigned s = row / (unsigned)a.parts;
+    return norm_place(a, v, s, (int)(row - s * a.parts), (int)(b - row * a.chunks));
 }
 
-// silu'(z) and friends.  v_exp_f32 and v_rcp_f32 are good to about one unit in
-// the last place of fp32, below the rounding of z itself.
+// A quad's rows that belong to the sample: [lo, hi) of 0..3.
+struct QuadRows {
+    int lo, hi;
+};
+__device__ __forceinline__ QuadRows quad_rows(const NormPlace& p, int64_t q) {
+    QuadRows r;
+    r.lo = p.f0 > 4 * q ? (int)(p.f0 - 4 * q) : 0;
+    r.hi = p.f1 < 4 * q + 4 ? (int)(p.f1 - 4 * q) : 4;
+    return r;
+}
+
+// The four vectors of a quad.  Rows outside the sample read its nearest row, so
+// that every load is in bounds without a branch.
+template <typename T, int V>
+struct Quad {
+    Raw<T, V> row[4];
+
+    __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, const NormPlace& p, int64_t q,
+                                         const QuadRows& in) {
+        const T* at = base + (4 * q - p.f0) * ld;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = r < in.lo ? in.lo : r >= in.hi ? in.hi - 1 : r;
+            row[r] = load_raw<T, V>(at + k * ld);
+        }
+    }
+};
+
+template <typename F>
+__device__ __forceinline__ F lane_xor(F v, int o) {
+    return __shfl_xor(v, o);
+}
+template <>
+__device__ __forceinline__ float2 lane_xor<float2>(float2 v, int o) {
+    return make_float2(__shfl_xor(v.x, o), __shfl_xor(v.y, o));
+}
+
+// Σ over each group of the chunk of a value per thread, in a fixed order; every
+// thread gets its own group's sum.  red: one value per thread, then one per
+// group behind them.
+template <typename F, int NT>
+__device__ __forceinline__ F group_sum(F v, const NormArgs& a, const NormPlace& p, F* red, int threads) {
+    const int per = a.sub == 1 ? a.lanes / a.lpg : 1;
+    const int members = a.ty * a.lpg;
+    int team = kWave;  // lanes per group: a power of two, no more than there are members
+    while (team > 1 && team / 2 >= members) team /= 2;
+    __syncthreads();
+    red[threadIdx.x] = v;
+    __syncthreads();
+    const int lane = threadIdx.x & (team - 1);
+    for (int g = threadIdx.x / team; g < per; g += threads / team) {
+        F sum{};
+        for (int i = lane; i < members; i += team) {
+            const int r = (int)((unsigned)i / (unsigned)a.lpg);
+            sum += red[r * a.lanes + g * a.lpg + (i - r * a.lpg)];
+        }
+        for (int o = team / 2; o > 0; o >>= 1) sum += lane_xor(sum, o);
+        if (lane == 0) red[NT + g] = sum;
+    }
+    __syncthreads();
+    const int g = a.sub == 1 ? p.tx / a.lpg : 0;
+    return red[NT + g];
+}
+
+// The masks of a slab thread's Q quads, drawn before the rows are loaded: the
+// column products of the generator and the rows together would not fit the
+// registers of a block of 1024 threads.
+template <int V, int Q>
+__device__ __forceinline__ void slab_masks(const NormArgs& a, const NormPlace& p, uint32_t (&bits)[Q]) {
+    ColumnKeep<V> columns;
+    columns.init(a.key, (uint32_t)p.c0);
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        bool kept[4][V];
+        columns.quad(a.key, (uint32_t)(p.q0 + p.ty + k * a.ty), kept);
+        bits[k] = pack_kept<V>(kept);
+        asm volatile("" : "+v"(bits[k]));  // a word from here on, not its 4 V comparisons
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// v_exp_f32 and v_rcp_f32 are good to about one unit in the last place of fp32,
+// below the rounding of z itself.
 __device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 template <int ACT>
@@ -161,7 +181,29 @@ __device__ __forceinline__ float act_grad(float z) {
     return 1.f;
 }
 
-// Calls f with an integral constant for the activation.
+// γ, β of a thread's channels.
+template <int V>
+struct NormParams {
+    float w[V], b[V];
+
+    __device__ __forceinline__ void load(const NormArgs& a, int c0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            w[e] = 1.f;
+            b[e] = 0.f;
+        }
+        if (a.weight) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e] = load_param(a.weight, a.ptype, c0 + e);
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) b[e] = load_param(a.bias, a.ptype, c0 + e);
+        }
+    }
+};
+
+// Calls f with an integral constant for the activation / the vector width.
 template <typename F>
 inline int with_act(int act, F&& f) {
     if (act == LDS_ACT_NONE) return f(IntC<LDS_ACT_NONE>{});
@@ -185,38 +227,103 @@ inline bool norm_sizes_ok(int64_t samples, int64_t n, int c, int groups) {
     return samples * n <= (int64_t)0x7fffffff;
 }
 
-constexpr int kNormBlocks = 2048;  // blocks of a pass: eight per CU
+inline int norm_elem(int dtype) { return dtype == LDS_F32 ? 4 : 2; }
 
-// Row parts per sample: about `want` blocks in all, and not less than eight
-// quads to a thread where there are that many.
-inline void norm_parts(int64_t samples, int64_t n, const NormCut& k, int want, int* parts, int64_t* part_q) {
+// How a call runs: the geometry of NormArgs, the block size, the form.
+struct NormPlan {
+    int v;
+    bool slab;
+    int threads;   // slab: 64 .. slab_threads
+    int quads;     // slab: row quads per thread, 1, 2 or 4
+    NormArgs a;
+};
+
+// slab_threads: the largest slab block.
+inline NormPlan norm_plan(int64_t samples, int64_t n, int c, int groups, int dtype, int slab_threads) {
+    NormPlan k{};
+    NormArgs& a = k.a;
+    const int elem = norm_elem(dtype);
+    a.samples = samples;
+    a.n = n;
+    a.c = c;
+    a.groups = groups;
+    a.cg = c / groups;
+    // the widest vector (<= 16 bytes) that lies in one group
+    k.v = 16 / elem;
+    while (k.v > 1 && a.cg % k.v) k.v /= 2;
+    const int lpg = a.cg / k.v;
     const int64_t quads = n / 4 + 2;  // a sample's quads, its partial first and last one among them
-    int64_t p = want / (samples * k.chunks > 0 ? samples * k.chunks : 1);
-    const int64_t most = (quads + 8 * k.ty - 1) / (8 * k.ty);
+    a.part_q = quads;
+    a.parts = 1;
+    a.sub = 1;
+    a.lpg = lpg;
+    const auto held = [&](int threads, int per) -> int64_t {  // quads per thread
+        const int ty = threads / (per * lpg);
+        return ty < 1 ? INT64_MAX : (quads + ty - 1) / ty;
+    };
+    if (lpg <= slab_threads && held(slab_threads, 1) <= kSlabQuads) {
+        k.slab = true;
+        // as few groups a block as there are, for more blocks; more where a
+        // row's share would be under a 64-byte line and blocks abound
+        int per = 1;
+        while (per * 2 <= groups && per * a.cg * elem < 64 && samples * (groups / (per * 2)) >= 512 &&
+               held(slab_threads, per * 2) <= kSlabQuads)
+            per *= 2;
+        // one wave where it holds the slab in one go, else the size at which a
+        // thread holds one quad
+        k.threads = 64;
+        while (k.threads < slab_threads && held(k.threads, per) > 1) k.threads *= 2;
+        const int64_t q = held(k.threads, per);
+        k.quads = q <= 1 ? 1 : q <= 2 ? 2 : 4;
+        a.lanes = per * lpg;
+        a.ty = k.threads / a.lanes;
+        a.chunks = (groups + per - 1) / per;
+        return k;
+    }
+    if (lpg <= kNormThreads) {
+        int per = kNormThreads / lpg;
+        if (per > groups) per = groups;
+        a.chunks = (groups + per - 1) / per;
+        per = (groups + a.chunks - 1) / a.chunks;  // even chunks
+        a.chunks = (groups + per - 1) / per;
+        a.lanes = per * lpg;
+    } else {
+        a.sub = (lpg + kNormThreads - 1) / kNormThreads;
+        a.lanes = (lpg + a.sub - 1) / a.sub;
+        a.lpg = a.lanes;
+        a.chunks = groups * a.sub;
+    }
+    a.ty = kNormThreads / a.lanes;
+    // about kNormBlocks blocks in all, and not less than two quads to a thread
+    // where there are that many
+    int64_t p = kNormBlocks / (samples * a.chunks > 0 ? samples * a.chunks : 1);
+    const int64_t most = (quads + 2 * a.ty - 1) / (2 * a.ty);
     if (p > most) p = most;
     if (p < 1) p = 1;
-    *part_q = (quads + p - 1) / p;
-    *parts = (int)((quads + *part_q - 1) / *part_q);
+    a.part_q = (quads + p - 1) / p;
+    a.parts = (int)((quads + a.part_q - 1) / a.part_q);
+    return k;
 }
 
-inline void norm_fill(NormArgs* a, const NormCut& k, int64_t samples, int64_t n, int c, int groups, int64_t sx,
-                      int64_t ldx, const void* weight, const void* bias, int ptype) {
-    a->samples = samples;
-    a->n = n;
-    a->sx = sx;
-    a->ldx = ldx;
-    a->c = c;
-    a->groups = groups;
-    a->cg = c / groups;
-    a->lanes = k.lanes;
-    a->ty = k.ty;
-    a->chunks = k.chunks;
-    a->lpg = k.lpg;
-    a->sub = k.sub;
-    norm_parts(samples, n, k, kNormBlocks, &a->parts, &a->part_q);
-    a->weight = weight;
-    a->bias = bias;
-    a->ptype = ptype;
+// Workspace of the backward: the channel sums of every part (of every sample,
+// in the slab form), then (parts) the two means of every group.
+inline int64_t backward_ws(const NormArgs& a, bool slab) {
+    if (slab) return a.samples == 1 ? 0 : a.samples * (int64_t)a.c * 8;
+    return a.samples * a.parts * (int64_t)a.c * 8 + a.samples * a.groups * 8;
+}
+
+// Blocks of a slab launch, and a block's place in it: the blocks of a sample
+// share its lines where a group is narrow, so from eight samples on a sample
+// stays on one XCD (blocks go round the eight of them).
+inline int64_t slab_blocks(const NormArgs& a) {
+    return a.samples >= 8 ? (a.samples + 7) / 8 * 8 * a.chunks : a.samples * a.chunks;
+}
+__device__ __forceinline__ bool slab_place(const NormArgs& a, int64_t& s, int& chunk) {
+    const unsigned b = blockIdx.x, u = a.samples >= 8 ? b >> 3 : b;
+    const unsigned t = u / (unsigned)a.chunks;
+    chunk = (int)(u - t * a.chunks);
+    s = a.samples >= 8 ? (int64_t)t * 8 + (b & 7) : t;
+    return s < a.samples;
 }
 
 }  // namespace lds

@@ -3,38 +3,182 @@
 //
 //   h = dy · mask · act'(z),  dβ_c = Σ h,  dγ_c = Σ h x̂,
 //   dx = r (γ h - mean_g(γ h) - x̂ mean_g(γ h x̂))
-// Three launches: the per-channel sums of every row part; the group means and
-// dγ / dβ from them; the elementwise pass.  z, x̂ and the mask are recomputed.
+// z, x̂ and the mask are recomputed from x, the statistics and the key.
 #include "norm.hpp"
 
 namespace lds {
 
+// x̂ and h of a quad.
 template <typename T, int V, int ACT, bool DROP>
-struct NormBack {
-    float mu, rs;
-    float w[V], b[V];
+struct BackQuad {
+    float xh[4][V], h[4][V];
 
-    __device__ __forceinline__ void load(const NormArgs& a, const NormPlace& p, const float* mean,
-                                         const float* rstd) {
-        mu = mean[p.s * a.groups + p.group];
-        rs = rstd[p.s * a.groups + p.group];
+    __device__ __forceinline__ void eval(const Quad<T, V>& x, const Quad<T, V>& g, const NormParams<V>& par, float mu,
+                                         float rs, const bool (&kept)[4][V], float scale) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            w[e] = a.weight ? load_param(a.weight, a.ptype, p.c0 + e) : 1.f;
-            b[e] = a.bias ? load_param(a.bias, a.ptype, p.c0 + e) : 0.f;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                xh[r][e] = (elem<T, V>(x.row[r], e) - mu) * rs;
+                float d = elem<T, V>(g.row[r], e);
+                if constexpr (DROP) d = kept[r][e] ? d * scale : 0.f;
+                if constexpr (ACT == LDS_ACT_RELU) {
+                    d = __builtin_fmaf(xh[r][e], par.w[e], par.b[e]) <= 0.f ? 0.f : d;
+                } else if constexpr (ACT != LDS_ACT_NONE) {
+                    d *= act_grad<ACT>(__builtin_fmaf(xh[r][e], par.w[e], par.b[e]));
+                }
+                h[r][e] = d;
+            }
+    }
+    __device__ __forceinline__ void sums(const QuadRows& in, float (&sh)[V], float (&sx)[V]) const {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (r < in.lo || r >= in.hi) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sh[e] += h[r][e];
+                sx[e] = __builtin_fmaf(h[r][e], xh[r][e], sx[e]);
+            }
         }
     }
-    // x -> x̂, g -> h
-    __device__ __forceinline__ void eval(float& x, float& g, int e, bool kept, float scale) const {
-        x = (x - mu) * rs;
-        if constexpr (DROP) g = kept ? g * scale : 0.f;
-        if constexpr (ACT == LDS_ACT_RELU) {
-            g = __builtin_fmaf(x, w[e], b[e]) <= 0.f ? 0.f : g;
-        } else if constexpr (ACT != LDS_ACT_NONE) {
-            g *= act_grad<ACT>(__builtin_fmaf(x, w[e], b[e]));
+    __device__ __forceinline__ void store(const QuadRows& in, const NormParams<V>& par, float rs, float m1, float m2,
+                                          T* __restrict__ at, int64_t ld) const {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (r < in.lo || r >= in.hi) continue;
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = rs * (__builtin_fmaf(par.w[e], h[r][e], -m1) - xh[r][e] * m2);
+            store_vec<T, V>(at + r * ld, o);
         }
     }
 };
+
+// The two sums of every channel of a block's chunk over its ty rows: value
+// i of a thread at red[i][thread], V values at a time.  Channel i of the chunk
+// is summed by a team of lanes in a fixed order; f(i, h, hx).
+template <int V, int NT, typename F>
+__device__ __forceinline__ void channel_sums(const float (&sh)[V], const float (&sx)[V], const NormArgs& a,
+                                             float2 (*red)[NT], int threads, F&& f) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) red[e][threadIdx.x] = make_float2(sh[e], sx[e]);
+    __syncthreads();
+    const int channels = a.lanes * V;
+    int team = 16;
+    while (team > 1 && (team / 2 >= a.ty || channels * team > 2 * threads)) team /= 2;
+    const int lane = threadIdx.x & (team - 1);
+    for (int i = threadIdx.x / team; i < channels; i += threads / team) {
+        float h = 0.f, hx = 0.f;
+        for (int r = lane; r < a.ty; r += team) {
+            const float2 t = red[i % V][r * a.lanes + i / V];
+            h += t.x;
+            hx += t.y;
+        }
+        for (int o = team / 2; o > 0; o >>= 1) {
+            h += __shfl_xor(h, o);
+            hx += __shfl_xor(hx, o);
+        }
+        if (lane == 0) f(i, h, hx);
+    }
+}
+
+// The chunk's first channel and the end of those it may write.
+__device__ __forceinline__ int chunk_first(const NormArgs& a, int chunk, int v) {
+    return a.sub == 1 ? chunk * a.lanes * v : (chunk / a.sub) * a.cg + (chunk % a.sub) * a.lanes * v;
+}
+__device__ __forceinline__ int chunk_last(const NormArgs& a, int chunk) {
+    return a.sub == 1 ? a.c : (chunk / a.sub + 1) * a.cg;
+}
+
+// ---------------------------------------------------------------------------
+// slab: x and dy in registers, Q quads a thread
+// ---------------------------------------------------------------------------
+
+template <typename T, int V, int ACT, bool DROP, int Q>
+__global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
+    const T* __restrict__ dy, int64_t sdy, int64_t lddy, const T* __restrict__ x, NormArgs a,
+    const float* __restrict__ mean, const float* __restrict__ rstd, float2* __restrict__ sums,
+    float* __restrict__ dweight, float* __restrict__ dbias, T* __restrict__ dx) {
+    constexpr int NT = kBackwardSlabThreads;
+    __shared__ float2 chan[V][NT];
+    __shared__ float2 red[2 * NT];
+    int64_t s;
+    int chunk;
+    if (!slab_place(a, s, chunk)) return;
+    const NormPlace p = norm_place(a, V, s, 0, chunk);
+    const T* xs = x + s * a.sx + p.c0;
+    const T* gs = dy + s * sdy + p.c0;
+    uint32_t masks[Q];
+    if constexpr (DROP) slab_masks<V, Q>(a, p, masks);
+    Quad<T, V> v[Q], g[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (p.live && q < p.q1) {
+            const QuadRows in = quad_rows(p, q);
+            v[k].load(xs, a.ldx, p, q, in);
+            g[k].load(gs, lddy, p, q, in);
+        }
+    }
+    float mu = 0.f, rs = 0.f;
+    NormParams<V> par{};
+    float sh[V] = {}, sx[V] = {};
+    if (p.live) {
+        mu = mean[s * a.groups + p.group];
+        rs = rstd[s * a.groups + p.group];
+        par.load(a, p.c0);
+    }
+    BackQuad<T, V, ACT, DROP> b;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (!p.live || q >= p.q1) continue;
+        bool kept[4][V];
+        if constexpr (DROP) unpack_kept<V>(masks[k], kept);
+        b.eval(v[k], g[k], par, mu, rs, kept, a.key.scale);
+        b.sums(quad_rows(p, q), sh, sx);
+    }
+    if (sums || dweight || dbias) {
+        const int c0 = chunk_first(a, chunk, V), c1 = chunk_last(a, chunk);
+        channel_sums<V, NT>(sh, sx, a, chan, blockDim.x, [&](int i, float h, float hx) {
+            if (c0 + i >= c1) return;
+            if (sums) {
+                sums[s * a.c + c0 + i] = make_float2(h, hx);
+            } else {  // one sample: the sums are the gradients
+                if (dbias) dbias[c0 + i] = h;
+                if (dweight) dweight[c0 + i] = hx;
+            }
+        });
+    }
+    if (!dx) return;
+    float2 m = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        m.x = __builtin_fmaf(par.w[e], sh[e], m.x);
+        m.y = __builtin_fmaf(par.w[e], sx[e], m.y);
+    }
+    m = group_sum<float2, NT>(m, a, p, red, blockDim.x);
+    const float inv = 1.f / ((float)a.n * (float)a.cg);
+    const float m1 = m.x * inv, m2 = m.y * inv;
+    if (!p.live) return;
+    T* ds = dx + p.c0;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (q >= p.q1) continue;
+        if constexpr (Q > 1) {
+            bool kept[4][V];
+            if constexpr (DROP) unpack_kept<V>(masks[k], kept);
+            b.eval(v[k], g[k], par, mu, rs, kept, a.key.scale);
+        }
+        b.store(quad_rows(p, q), par, rs, m1, m2, ds + 4 * q * a.c, a.c);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// parts
+// ---------------------------------------------------------------------------
 
 template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __restrict__ dy, int64_t sdy,
@@ -43,59 +187,36 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __re
                                                                    const float* __restrict__ rstd,
                                                                    float2* __restrict__ out) {
     __shared__ float2 red[V][kNormThreads];
-    const NormPlace p = norm_place(a, V);
+    const NormPlace p = norm_part_place(a, V);
     float sh[V] = {}, sx[V] = {};
     if (p.live) {
-        NormBack<T, V, ACT, DROP> k;
-        k.load(a, p, mean, rstd);
+        const float mu = mean[p.s * a.groups + p.group], rs = rstd[p.s * a.groups + p.group];
+        NormParams<V> par;
+        par.load(a, p.c0);
+        ColumnKeep<V> columns;
+        if constexpr (DROP) columns.init(a.key, (uint32_t)p.c0);
         const T* xs = x + p.s * a.sx + p.c0;
         const T* gs = dy + p.s * sdy + p.c0;
-        for (int64_t q = p.q0 + p.row0; q < p.q1; q += p.stride) {
-            float v[4][V], g[4][V];
-            bool in[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t f = 4 * q + r;
-                in[r] = f >= p.f0 && f < p.f1;
-                if (in[r]) {
-                    load_vec<T, V>(xs + (f - p.f0) * a.ldx, v[r]);
-                    load_vec<T, V>(gs + (f - p.f0) * lddy, g[r]);
-                }
-            }
-            const uint32_t keep = DROP ? keep_bits<V>(a.key, (uint32_t)p.c0, (uint32_t)q) : 0u;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (!in[r]) continue;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    k.eval(v[r][e], g[r][e], e, (keep >> (4 * e + r)) & 1u, a.key.scale);
-                    sh[e] += g[r][e];
-                    sx[e] = __builtin_fmaf(g[r][e], v[r][e], sx[e]);
-                }
-            }
+        for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
+            const QuadRows in = quad_rows(p, q);
+            Quad<T, V> v, g;
+            v.load(xs, a.ldx, p, q, in);
+            g.load(gs, lddy, p, q, in);
+            BackQuad<T, V, ACT, DROP> b;
+            bool kept[4][V];
+            if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
+            b.eval(v, g, par, mu, rs, kept, a.key.scale);
+            b.sums(in, sh, sx);
         }
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) red[e][threadIdx.x] = make_float2(sh[e], sx[e]);
-    __syncthreads();
-    // the ty rows of every channel of the chunk, a thread per channel
-    const int first = a.sub == 1 ? p.chunk * a.lanes * V
-                                 : (p.chunk / a.sub) * a.cg + (p.chunk % a.sub) * a.lanes * V;
-    const int last = a.sub == 1 ? a.c : (p.chunk / a.sub + 1) * a.cg;
-    for (int i = threadIdx.x; i < a.lanes * V; i += kNormThreads) {
-        if (first + i >= last) break;
-        float h = 0.f, hx = 0.f;
-        for (int r = 0; r < a.ty; ++r) {
-            const float2 t = red[i % V][r * a.lanes + i / V];
-            h += t.x;
-            hx += t.y;
-        }
-        out[(p.s * a.parts + p.part) * a.c + first + i] = make_float2(h, hx);
-    }
+    const int c0 = chunk_first(a, p.chunk, V), c1 = chunk_last(a, p.chunk);
+    channel_sums<V, kNormThreads>(sh, sx, a, red, kNormThreads, [&](int i, float h, float hx) {
+        if (c0 + i < c1) out[(p.s * a.parts + p.part) * a.c + c0 + i] = make_float2(h, hx);
+    });
 }
 
-// Blocks [0, pairs): a (sample, group)'s two means.  The blocks after them:
-// 16 channels each, summed over every sample and part.
+// Blocks [0, pairs): a (sample, group)'s two means.  The blocks after them: four
+// channels each, summed over every sample and part.
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const float2* __restrict__ sums, NormArgs a,
                                                                       int64_t pairs, float2* __restrict__ means,
                                                                       float* __restrict__ dweight,
@@ -107,8 +228,9 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
         const int64_t s = blockIdx.x / a.groups;
         const int g = (int)(blockIdx.x - s * a.groups);
         const int64_t items = (int64_t)a.parts * a.cg;
+#pragma unroll 4
         for (int64_t i = t; i < items; i += kNormThreads) {
-            const int64_t part = i / a.cg;
+            const int64_t part = (uint32_t)i / (uint32_t)a.cg;
             const int c = g * a.cg + (int)(i - part * a.cg);
             const float2 v = sums[(s * a.parts + part) * a.c + c];
             const float w = a.weight ? load_param(a.weight, a.ptype, c) : 1.f;
@@ -129,24 +251,28 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
         }
         return;
     }
-    const int c = (int)(blockIdx.x - pairs) * 16 + (t & 15);
+    const int c = (int)(blockIdx.x - pairs) * 4 + (t & 3);
     const int64_t rows = a.samples * a.parts;
-    if (c < a.c)
-        for (int64_t i = t >> 4; i < rows; i += kNormThreads / 16) {
+    if (c < a.c) {
+#pragma unroll 4
+        for (int64_t i = t >> 2; i < rows; i += kNormThreads / 4) {
             const float2 v = sums[i * a.c + c];
             h += (double)v.x;
             hx += (double)v.y;
         }
-    red[0][t] = h;
-    red[1][t] = hx;
+    }
+    for (int o = 4; o < kWave; o <<= 1) {  // the wave's 16 rows
+        h += __shfl_xor(h, o);
+        hx += __shfl_xor(hx, o);
+    }
+    if (wave_lane() < 4) {
+        red[0][wave_id() * 4 + (t & 3)] = h;
+        red[1][wave_id() * 4 + (t & 3)] = hx;
+    }
     __syncthreads();
-    if (t < 16 && c < a.c) {
-        for (int i = t + 16; i < kNormThreads; i += 16) {
-            h += red[0][i];
-            hx += red[1][i];
-        }
-        if (dbias) dbias[c] = (float)h;
-        if (dweight) dweight[c] = (float)hx;
+    if (t < 4 && c < a.c) {
+        if (dbias) dbias[c] = (float)(red[0][t] + red[0][4 + t] + red[0][8 + t] + red[0][12 + t]);
+        if (dweight) dweight[c] = (float)(red[1][t] + red[1][4 + t] + red[1][8 + t] + red[1][12 + t]);
     }
 }
 
@@ -157,37 +283,27 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
                                                                  const float* __restrict__ rstd,
                                                                  const float2* __restrict__ means,
                                                                  T* __restrict__ dx) {
-    const NormPlace p = norm_place(a, V);
+    const NormPlace p = norm_part_place(a, V);
     if (!p.live) return;
-    NormBack<T, V, ACT, DROP> k;
-    k.load(a, p, mean, rstd);
+    const float mu = mean[p.s * a.groups + p.group], rs = rstd[p.s * a.groups + p.group];
+    NormParams<V> par;
+    par.load(a, p.c0);
+    ColumnKeep<V> columns;
+    if constexpr (DROP) columns.init(a.key, (uint32_t)p.c0);
     const float2 m = means[p.s * a.groups + p.group];
     const T* xs = x + p.s * a.sx + p.c0;
     const T* gs = dy + p.s * sdy + p.c0;
-    T* ds = dx + p.f0 * a.c + p.c0;
-    for (int64_t q = p.q0 + p.row0; q < p.q1; q += p.stride) {
-        float v[4][V], g[4][V];
-        bool in[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t f = 4 * q + r;
-            in[r] = f >= p.f0 && f < p.f1;
-            if (in[r]) {
-                load_vec<T, V>(xs + (f - p.f0) * a.ldx, v[r]);
-                load_vec<T, V>(gs + (f - p.f0) * lddy, g[r]);
-            }
-        }
-        const uint32_t keep = DROP ? keep_bits<V>(a.key, (uint32_t)p.c0, (uint32_t)q) : 0u;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (!in[r]) continue;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                k.eval(v[r][e], g[r][e], e, (keep >> (4 * e + r)) & 1u, a.key.scale);
-                v[r][e] = k.rs * (__builtin_fmaf(k.w[e], g[r][e], -m.x) - v[r][e] * m.y);
-            }
-            store_vec<T, V>(ds + (4 * q + r - p.f0) * a.c, v[r]);
-        }
+    T* ds = dx + p.c0;
+    for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
+        const QuadRows in = quad_rows(p, q);
+        Quad<T, V> v, g;
+        v.load(xs, a.ldx, p, q, in);
+        g.load(gs, lddy, p, q, in);
+        BackQuad<T, V, ACT, DROP> b;
+        bool kept[4][V];
+        if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
+        b.eval(v, g, par, mu, rs, kept, a.key.scale);
+        b.store(in, par, rs, m.x, m.y, ds + 4 * q * a.c, a.c);
     }
 }
 
@@ -206,38 +322,58 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
     LDS_CHECK_ARG(act >= LDS_ACT_NONE && act <= LDS_ACT_SILU && dtype >= LDS_F32 && dtype <= LDS_F16);
     // with no rows the sums are the caller's zeros to write
     if (samples == 0 || n == 0 || c == 0) return 0;
-    LDS_CHECK_ARG(dy && x && mean && rstd && ws && ldx >= c && lddy >= c);
+    LDS_CHECK_ARG(dy && x && mean && rstd && ldx >= c && lddy >= c);
     LDS_CHECK_ARG(samples == 1 || (sx >= 0 && sdy >= 0));
+    if (!dx && !dweight && !dbias) return 0;
     hipStream_t st = (hipStream_t)stream;
-    NormArgs a{};
+    NormPlan k = norm_plan(samples, n, c, groups, dtype, kBackwardSlabThreads);
+    NormArgs& a = k.a;
+    LDS_CHECK_ARG(ws || backward_ws(a, k.slab) == 0);
     const bool drop = keep_prob < 1.f && drop_key(keep_prob, scale, seed, tag, counter, &a.key);
-    const int v = norm_vec(c, groups, dtype == LDS_F32 ? 4 : 2);
-    const NormCut k = norm_cut(c, groups, v);
-    norm_fill(&a, k, samples, n, c, groups, sx, ldx, weight, bias, ptype);
-    const int64_t blocks = samples * a.parts * a.chunks;
-    const int64_t pairs = dx ? samples * groups : 0;
-    const int64_t cblocks = pairs + ((dweight || dbias) ? (c + 15) / 16 : 0);
+    a.sx = sx;
+    a.ldx = ldx;
+    a.weight = weight;
+    a.bias = bias;
+    a.ptype = ptype;
+    const int64_t blocks = k.slab ? slab_blocks(a) : samples * a.parts * a.chunks;
+    const int64_t pairs = dx && !k.slab ? samples * groups : 0;
+    const bool params = dweight || dbias;
+    const int64_t cblocks = pairs + (params && !(k.slab && samples == 1) ? (c + 3) / 4 : 0);
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && cblocks < (int64_t)1 << 31);
-    if (cblocks == 0) return 0;
     float2* sums = (float2*)ws;
-    float2* means = sums + samples * a.parts * (int64_t)c;
+    float2* means = k.slab ? nullptr : sums + samples * a.parts * (int64_t)c;
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
-        return with_vec<16 / (int)sizeof(T)>(v, [&](auto vc) -> int {
+        return with_vec<16 / (int)sizeof(T)>(k.v, [&](auto vc) -> int {
             constexpr int V = decltype(vc)::value;
             return with_act(act, [&](auto ac) -> int {
                 constexpr int ACT = decltype(ac)::value;
                 auto go = [&](auto dr) {
                     constexpr bool DROP = decltype(dr)::value;
-                    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
-                                       dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
-                                       rstd, sums);
-                    hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3((unsigned)cblocks), dim3(kNormThreads), 0, st,
-                                       sums, a, pairs, means, dweight, dbias);
-                    if (dx)
+                    auto slab = [&](auto qc) {
+                        const bool direct = samples == 1;
+                        hipLaunchKernelGGL((gn_bwd_slab_kernel<T, V, ACT, DROP, decltype(qc)::value>),
+                                           dim3((unsigned)blocks), dim3(k.threads), 0, st, (const T*)dy, sdy, lddy,
+                                           (const T*)x, a, mean, rstd, params && !direct ? sums : nullptr,
+                                           direct ? dweight : nullptr, direct ? dbias : nullptr, (T*)dx);
+                    };
+                    if (!k.slab)
+                        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
+                                           dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
+                                           rstd, sums);
+                    else if (k.quads == 1)
+                        slab(IntC<1>{});
+                    else if (k.quads == 2)
+                        slab(IntC<2>{});
+                    else
+                        slab(IntC<4>{});
+                    if (cblocks)
+                        hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3((unsigned)cblocks), dim3(kNormThreads), 0, st,
+                                           (const float2*)sums, a, pairs, means, dweight, dbias);
+                    if (!k.slab && dx)
                         hipLaunchKernelGGL((gn_bwd_dx_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
                                            dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
-                                           rstd, means, (T*)dx);
+                                           rstd, (const float2*)means, (T*)dx);
                 };
                 drop ? go(BoolC<true>{}) : go(BoolC<false>{});
                 LDS_RETURN_LAST_ERROR();

@@ -1,8 +1,5 @@
 // Group norm + activation + keyed dropout, channels last, forward
 // (include/ldsgnn.h lds_group_norm_forward).
-//
-// Three launches: (count, mean, centred squares) of every row part and group;
-// their combination per (sample, group); the elementwise pass.
 #include "norm.hpp"
 
 namespace lds {
@@ -12,6 +9,108 @@ struct Moments {
     float count, m2;
 };
 
+// y of a quad from x: z = ((x - mean) rstd) γ + β.
+template <typename T, int V, int ACT, bool DROP>
+__device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& in, const NormParams<V>& par, float mu,
+                                           float rs, const bool (&kept)[4][V], float scale, T* __restrict__ at,
+                                           int64_t ld) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (r < in.lo || r >= in.hi) continue;
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float z = __builtin_fmaf((elem<T, V>(x.row[r], e) - mu) * rs, par.w[e], par.b[e]);
+            o[e] = act_f<ACT>(z);
+            if constexpr (DROP) o[e] = kept[r][e] ? o[e] * scale : 0.f;
+        }
+        store_vec<T, V>(at + r * ld, o);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// slab: one block, a sample's rows of a few groups, Q quads a thread
+// ---------------------------------------------------------------------------
+
+template <typename T, int V, int ACT, bool DROP, int Q>
+__global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, NormArgs a, float eps,
+                                                       T* __restrict__ y, float* __restrict__ mean,
+                                                       float* __restrict__ rstd) {
+    __shared__ float2 red[2 * 1024];
+    int64_t s;
+    int chunk;
+    if (!slab_place(a, s, chunk)) return;
+    const NormPlace p = norm_place(a, V, s, 0, chunk);
+    const T* xs = x + s * a.sx + p.c0;
+    uint32_t masks[Q];
+    if constexpr (DROP) slab_masks<V, Q>(a, p, masks);
+    Quad<T, V> v[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (p.live && q < p.q1) v[k].load(xs, a.ldx, p, q, quad_rows(p, q));
+    }
+    // The mean of the values about the group's first one, so that an offset of
+    // the data costs no digits; then, about that mean, the squares and what
+    // the mean is still off by (the first value may be an outlier).
+    const float first = p.live ? (float)x[s * a.sx + (int64_t)p.group * a.cg] : 0.f;
+    const float inv = 1.f / ((float)a.n * (float)a.cg);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (!p.live || q >= p.q1) continue;
+        const QuadRows in = quad_rows(p, q);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r >= in.lo && r < in.hi) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum += elem<T, V>(v[k].row[r], e) - first;
+            }
+    }
+    const float m0 = first + group_sum<float, 1024>(sum, a, p, (float*)red, blockDim.x) * inv;
+    float2 d2 = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (!p.live || q >= p.q1) continue;
+        const QuadRows in = quad_rows(p, q);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r >= in.lo && r < in.hi) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float d = elem<T, V>(v[k].row[r], e) - m0;
+                    d2.x += d;
+                    d2.y = __builtin_fmaf(d, d, d2.y);
+                }
+            }
+    }
+    d2 = group_sum<float2, 1024>(d2, a, p, red, blockDim.x);
+    const float off = d2.x * inv, mu = m0 + off;
+    const float rs = 1.f / sqrtf(fmaxf(__builtin_fmaf(-off, off, d2.y * inv), 0.f) + eps);
+    if (!p.live) return;
+    if (p.ty == 0 && p.c0 == p.group * a.cg) {
+        mean[s * a.groups + p.group] = mu;
+        rstd[s * a.groups + p.group] = rs;
+    }
+    NormParams<V> par;
+    par.load(a, p.c0);
+    T* ys = y + p.c0;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const int64_t q = p.q0 + p.ty + k * a.ty;
+        if (q >= p.q1) continue;
+        bool kept[4][V];
+        if constexpr (DROP) unpack_kept<V>(masks[k], kept);
+        apply_quad<T, V, ACT, DROP>(v[k], quad_rows(p, q), par, mu, rs, kept, a.key.scale, ys + 4 * q * a.c, a.c);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// parts
+// ---------------------------------------------------------------------------
+
 // Statistics of one part.  A thread takes the 4 V values of a row quad at a
 // time: their mean, about the first of them, then the squares about that mean,
 // then one merge into the thread's running moments,
@@ -19,58 +118,69 @@ struct Moments {
 // No difference of large sums is taken, so neither an offset of the data nor an
 // outlier costs digits; means are carried in fp64.
 template <typename T, int V>
+__device__ __forceinline__ void quad_moments(const Quad<T, V>& v, const QuadRows& in, double& mean, float& m2,
+                                             float& cnt) {
+    float f[4][V], s1 = 0.f, s2 = 0.f;
+    // rows outside the sample repeat its nearest row: out of the sums by a factor
+    const float k = elem<T, V>(v.row[0], 0);
+    const float m = (float)((in.hi - in.lo) * V);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float use = r >= in.lo && r < in.hi ? 1.f : 0.f;
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            f[r][e] = elem<T, V>(v.row[r], e) - k;
+            t += f[r][e];
+        }
+        s1 = __builtin_fmaf(t, use, s1);
+    }
+    const float mq = s1 * __builtin_amdgcn_rcpf(m);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float use = r >= in.lo && r < in.hi ? 1.f : 0.f;
+        float t = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = f[r][e] - mq;
+            t = __builtin_fmaf(d, d, t);
+        }
+        s2 = __builtin_fmaf(t, use, s2);
+    }
+    const double delta = ((double)k + (double)mq) - mean;
+    const float part = m * __builtin_amdgcn_rcpf(cnt + m);
+    mean += delta * (double)part;
+    m2 += __builtin_fmaf((float)delta * (float)delta, cnt * part, s2);
+    cnt += m;
+}
+
+template <typename T, int V>
 __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const T* __restrict__ x, NormArgs a,
                                                                 Moments* __restrict__ out) {
-    __shared__ double s_mean[kNormThreads];
-    __shared__ float s_cnt[kNormThreads], s_m2[kNormThreads];
-    const NormPlace p = norm_place(a, V);
+    __shared__ double red[2 * kNormThreads];
+    const NormPlace p = norm_part_place(a, V);
     double mean = 0.0;
     float m2 = 0.f, cnt = 0.f;
     if (p.live) {
         const T* xs = x + p.s * a.sx + p.c0;
-        for (int64_t q = p.q0 + p.row0; q < p.q1; q += p.stride) {
-            float v[4][V];
-            bool in[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t f = 4 * q + r;
-                in[r] = f >= p.f0 && f < p.f1;
-                if (in[r]) load_vec<T, V>(xs + (f - p.f0) * a.ldx, v[r]);
-            }
-            quad_moments<V>(v, in, mean, m2, cnt);
+#pragma unroll 2
+        for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
+            const QuadRows in = quad_rows(p, q);
+            Quad<T, V> v;
+            v.load(xs, a.ldx, p, q, in);
+            quad_moments<T, V>(v, in, mean, m2, cnt);
         }
     }
-    s_cnt[threadIdx.x] = cnt;
-    s_mean[threadIdx.x] = mean;
-    s_m2[threadIdx.x] = m2;
-    __syncthreads();
-    // one wave per group of the chunk over its ty x lpg threads
-    const int per = a.sub == 1 ? a.lanes / a.lpg : 1;
-    const int members = a.ty * a.lpg;
-    for (int gi = wave_id(); gi < per; gi += kNormThreads / kWave) {
-        const int g = a.sub == 1 ? p.chunk * per + gi : p.chunk / a.sub;
-        if (g >= a.groups) break;
-        float c = 0.f, g2 = 0.f;
-        double m = 0.0;
-        for (int i = wave_lane(); i < members; i += kWave) {
-            const int t = (i / a.lpg) * a.lanes + gi * a.lpg + i % a.lpg;
-            c += s_cnt[t];
-            m += (double)s_cnt[t] * s_mean[t];
-        }
-        c = wave_sum(c);
-        m = wave_sum(m);
-        const double gm = c > 0.f ? m / (double)c : 0.0;
-        for (int i = wave_lane(); i < members; i += kWave) {
-            const int t = (i / a.lpg) * a.lanes + gi * a.lpg + i % a.lpg;
-            const float d = (float)(s_mean[t] - gm);
-            g2 += s_cnt[t] > 0.f ? s_m2[t] + s_cnt[t] * d * d : 0.f;
-        }
-        g2 = wave_sum(g2);
-        if (wave_lane() == 0) {
-            const int j = p.part * a.sub + (a.sub == 1 ? 0 : p.chunk - g * a.sub);
-            out[(p.s * a.groups + g) * ((int64_t)a.parts * a.sub) + j] = Moments{gm, c, g2};
-        }
-    }
+    const double c = group_sum<double, kNormThreads>((double)cnt, a, p, red, kNormThreads);
+    const double gm =
+        group_sum<double, kNormThreads>((double)cnt * mean, a, p, red, kNormThreads) / (c > 0.0 ? c : 1.0);
+    const float d = (float)(mean - gm);
+    const double g2 = group_sum<double, kNormThreads>(cnt > 0.f ? (double)(m2 + cnt * d * d) : 0.0, a, p, red,
+                                                      kNormThreads);
+    const int at = a.sub == 1 ? 0 : p.chunk - p.group * a.sub;
+    if (p.live && p.ty == 0 && (a.sub == 1 ? p.tx % a.lpg == 0 : p.tx == 0))
+        out[(p.s * a.groups + p.group) * ((int64_t)a.parts * a.sub) + p.part * a.sub + at] =
+            Moments{gm, (float)c, (float)g2};
 }
 
 // One wave per (sample, group): its parts combined in fp64.
@@ -81,6 +191,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_combine_kernel(const Moments*
     if (i >= total) return;
     const Moments* m = in + i * parts;
     double c = 0.0, s = 0.0;
+#pragma unroll 4
     for (int j = wave_lane(); j < parts; j += kWave) {
         c += (double)m[j].count;
         s += (double)m[j].count * m[j].mean;
@@ -89,6 +200,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_combine_kernel(const Moments*
     s = wave_sum(s);
     const double mu = s / c;
     double v = 0.0;
+#pragma unroll 4
     for (int j = wave_lane(); j < parts; j += kWave) {
         const double d = m[j].mean - mu;
         v += m[j].count > 0.f ? (double)m[j].m2 + (double)m[j].count * d * d : 0.0;
@@ -104,40 +216,23 @@ template <typename T, int V, int ACT, bool DROP>
 __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restrict__ x, NormArgs a,
                                                                 const float* __restrict__ mean,
                                                                 const float* __restrict__ rstd, T* __restrict__ y) {
-    const NormPlace p = norm_place(a, V);
+    const NormPlace p = norm_part_place(a, V);
     if (!p.live) return;
     const float mu = mean[p.s * a.groups + p.group];
     const float rs = rstd[p.s * a.groups + p.group];
-    float w[V], b[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        w[e] = a.weight ? load_param(a.weight, a.ptype, p.c0 + e) : 1.f;
-        b[e] = a.bias ? load_param(a.bias, a.ptype, p.c0 + e) : 0.f;
-    }
+    NormParams<V> par;
+    par.load(a, p.c0);
+    ColumnKeep<V> columns;
+    if constexpr (DROP) columns.init(a.key, (uint32_t)p.c0);
     const T* xs = x + p.s * a.sx + p.c0;
-    T* ys = y + p.f0 * a.c + p.c0;
-    for (int64_t q = p.q0 + p.row0; q < p.q1; q += p.stride) {
-        float v[4][V];
-        bool in[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int64_t f = 4 * q + r;
-            in[r] = f >= p.f0 && f < p.f1;
-            if (in[r]) load_vec<T, V>(xs + (f - p.f0) * a.ldx, v[r]);
-        }
-        const uint32_t keep = DROP ? keep_bits<V>(a.key, (uint32_t)p.c0, (uint32_t)q) : 0u;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (!in[r]) continue;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float z = __builtin_fmaf((v[r][e] - mu) * rs, w[e], b[e]);
-                float o = act_f<ACT>(z);
-                if constexpr (DROP) o = (keep >> (4 * e + r)) & 1u ? o * a.key.scale : 0.f;
-                v[r][e] = o;
-            }
-            store_vec<T, V>(ys + (4 * q + r - p.f0) * a.c, v[r]);
-        }
+    T* ys = y + p.c0;
+    for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
+        const QuadRows in = quad_rows(p, q);
+        Quad<T, V> v;
+        v.load(xs, a.ldx, p, q, in);
+        bool kept[4][V];
+        if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
+        apply_quad<T, V, ACT, DROP>(v, in, par, mu, rs, kept, a.key.scale, ys + 4 * q * a.c, a.c);
     }
 }
 
@@ -145,22 +240,12 @@ __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restr
 
 using namespace lds;
 
-namespace {
-
-int elem_bytes(int dtype) { return dtype == LDS_F32 ? 4 : 2; }
-
-}  // namespace
-
 extern "C" int64_t lds_group_norm_ws_bytes(int64_t samples, int64_t n, int c, int groups, int dtype, int backward) {
     if (!norm_sizes_ok(samples, n, c, groups) || dtype < LDS_F32 || dtype > LDS_F16) return -1;
     if (samples == 0 || n == 0 || c == 0) return 0;
-    const NormCut k = norm_cut(c, groups, norm_vec(c, groups, elem_bytes(dtype)));
-    int parts;
-    int64_t part_q;
-    norm_parts(samples, n, k, kNormBlocks, &parts, &part_q);
-    if (!backward) return samples * groups * parts * k.sub * (int64_t)sizeof(Moments);
-    // per channel sums of the parts, then the two group means
-    return samples * parts * (int64_t)c * 8 + samples * groups * 8;
+    const NormPlan k = norm_plan(samples, n, c, groups, dtype, backward ? kBackwardSlabThreads : kForwardSlabThreads);
+    if (backward) return backward_ws(k.a, k.slab);
+    return k.slab ? 0 : samples * groups * k.a.parts * k.a.sub * (int64_t)sizeof(Moments);
 }
 
 extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, int64_t samples, int64_t n, int c,
@@ -171,33 +256,50 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     LDS_CHECK_ARG(keep_prob >= 0.f && ptype >= LDS_F32 && ptype <= LDS_F16);
     LDS_CHECK_ARG(act >= LDS_ACT_NONE && act <= LDS_ACT_SILU && dtype >= LDS_F32 && dtype <= LDS_F16);
     if (samples == 0 || n == 0 || c == 0) return 0;
-    LDS_CHECK_ARG(x && y && mean && rstd && ws && ldx >= c && (samples == 1 || sx >= 0));
+    LDS_CHECK_ARG(x && y && mean && rstd && ldx >= c && (samples == 1 || sx >= 0));
     hipStream_t st = (hipStream_t)stream;
-    NormArgs a{};
+    NormPlan k = norm_plan(samples, n, c, groups, dtype, kForwardSlabThreads);
+    NormArgs& a = k.a;
+    LDS_CHECK_ARG(k.slab || ws);
     const bool drop = keep_prob < 1.f && drop_key(keep_prob, scale, seed, tag, counter, &a.key);
-    const int v = norm_vec(c, groups, elem_bytes(dtype));
-    const NormCut k = norm_cut(c, groups, v);
-    norm_fill(&a, k, samples, n, c, groups, sx, ldx, weight, bias, ptype);
-    const int64_t blocks = samples * a.parts * a.chunks;
+    a.sx = sx;
+    a.ldx = ldx;
+    a.weight = weight;
+    a.bias = bias;
+    a.ptype = ptype;
+    const int64_t blocks = k.slab ? slab_blocks(a) : samples * a.parts * a.chunks;
     const int64_t pairs = samples * groups;
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && pairs < (int64_t)1 << 32);
-    Moments* mom = (Moments*)ws;
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
-        return with_vec<16 / (int)sizeof(T)>(v, [&](auto vc) -> int {
+        return with_vec<16 / (int)sizeof(T)>(k.v, [&](auto vc) -> int {
             constexpr int V = decltype(vc)::value;
-            hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0, st,
-                               (const T*)x, a, mom);
-            hipLaunchKernelGGL(gn_combine_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(kNormThreads), 0, st, mom,
-                               pairs, a.parts * a.sub, eps, mean, rstd);
+            if (!k.slab) {
+                hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0, st,
+                                   (const T*)x, a, (Moments*)ws);
+                hipLaunchKernelGGL(gn_combine_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(kNormThreads), 0, st,
+                                   (const Moments*)ws, pairs, a.parts * a.sub, eps, mean, rstd);
+            }
             return with_act(act, [&](auto ac) -> int {
                 constexpr int ACT = decltype(ac)::value;
-                if (drop)
-                    hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, true>), dim3((unsigned)blocks),
-                                       dim3(kNormThreads), 0, st, (const T*)x, a, mean, rstd, (T*)y);
-                else
-                    hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, false>), dim3((unsigned)blocks),
-                                       dim3(kNormThreads), 0, st, (const T*)x, a, mean, rstd, (T*)y);
+                auto go = [&](auto dr) {
+                    constexpr bool DROP = decltype(dr)::value;
+                    auto slab = [&](auto qc) {
+                        hipLaunchKernelGGL((gn_slab_kernel<T, V, ACT, DROP, decltype(qc)::value>),
+                                           dim3((unsigned)blocks), dim3(k.threads), 0, st, (const T*)x, a, eps, (T*)y,
+                                           mean, rstd);
+                    };
+                    if (!k.slab)
+                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
+                                           dim3(kNormThreads), 0, st, (const T*)x, a, mean, rstd, (T*)y);
+                    else if (k.quads == 1)
+                        slab(IntC<1>{});
+                    else if (k.quads == 2)
+                        slab(IntC<2>{});
+                    else
+                        slab(IntC<4>{});
+                };
+                drop ? go(BoolC<true>{}) : go(BoolC<false>{});
                 LDS_RETURN_LAST_ERROR();
             });
         });

@@ -77,27 +77,126 @@ __device__ __forceinline__ float load_param(const void* p, int code, int64_t i) 
     return (float)reinterpret_cast<const f16_t*>(p)[i];
 }
 
-// The mask of the RNG contract (include/ldsgnn.h) at V neighbouring columns
-// and the four rows of a row quad: bit (4 e + r) of the result is set where
-// u(4 rq + r, col + e) < keep.  u < keep is a comparison of whole numbers:
-// u = (w >> 8) 2^-24 < keep  <=>  w < ceil(keep 2^24) 256 = `thr` (keep < 1).
+// V consecutive elements as they lie in memory, and as fp32.
+template <typename T, int V>
+using Raw = typename VecOf<T, V>::type;
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* __restrict__ p) {
+    return *reinterpret_cast<const Raw<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ float elem(const Raw<T, V>& v, int e) {
+    if constexpr (V == 1)
+        return (float)v;
+    else
+        return (float)v[e];
+}
+
+// The mask of the RNG contract (include/ldsgnn.h): u(row, col) < keep, with
+// u = (w >> 8) 2^-24, as a comparison of whole numbers,
+// w < ceil(keep 2^24) 256 = `thr` (keep < 1).
 struct DropKey {
     uint32_t k0, k1, tag, counter, thr;
     float scale;
 };
 
+constexpr uint32_t kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u, kPhiloxW0 = 0x9E3779B9u,
+                   kPhiloxW1 = 0xBB67AE85u;
+
+__device__ __forceinline__ void mul_wide(uint32_t m, uint32_t x, uint32_t& hi, uint32_t& lo) {
+    uint64_t p, cc;  // one v_mad_u64_u32 (common.hpp philox4x32_10)
+    asm("v_mad_u64_u32 %0, %1, %2, %3, 0" : "=v"(p), "=s"(cc) : "s"(m), "v"(x));
+    (void)cc;
+    hi = (uint32_t)(p >> 32);
+    lo = (uint32_t)p;
+}
+
+// Philox4x32-10 at V neighbouring columns and any row quads.  Of the counter
+// (column, row quad, tag, draw) only the row quad changes along a thread's
+// rows, so the products of the first three rounds that do not see it are
+// taken once: 15.1 wide products a quad and column are left of 20.
+//   round 1:  a = (M1·tag hi ^ rq ^ k0,  M1·tag lo,  M0·col hi ^ draw ^ k1,  M0·col lo)
+//   round 2:  q0 = M0·a0 (row quad only),  q1 = M1·a2 (column only)
+//   round 3:  r0 = M0·(q1 hi ^ a1 ^ k0) (column only),  r1 = M1·(q0 hi ^ a3 ^ k1)
 template <int V>
-__device__ __forceinline__ uint32_t keep_bits(const DropKey& k, uint32_t col, uint32_t rq) {
+struct ColumnKeep {
+    uint32_t a3[V], b1[V], r0h[V], r0l[V];
+    uint32_t u0;
+
+    __device__ __forceinline__ void init(const DropKey& k, uint32_t col) {
+        uint32_t th, tl;
+        mul_wide(kPhiloxM1, k.tag, th, tl);
+        u0 = th ^ k.k0;
+        const uint32_t k0b = k.k0 + kPhiloxW0, k1b = k.k1 + kPhiloxW1;
+        const uint32_t k0c = k0b + kPhiloxW0, k1c = k1b + kPhiloxW1;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            uint32_t hi, lo, qh, ql, rh, rl;
+            mul_wide(kPhiloxM0, col + e, hi, lo);
+            a3[e] = lo ^ k1b;
+            mul_wide(kPhiloxM1, hi ^ k.counter ^ k.k1, qh, ql);
+            b1[e] = ql ^ k0c;
+            mul_wide(kPhiloxM0, qh ^ tl ^ k0b, rh, rl);
+            r0h[e] = rh ^ k1c;
+            r0l[e] = rl;
+        }
+    }
+
+    // kept[r][e]: the element of row 4 rq + r at column col + e is kept
+    __device__ __forceinline__ void quad(const DropKey& k, uint32_t rq, bool (&kept)[4][V]) const {
+        uint32_t qh, ql;
+        mul_wide(kPhiloxM0, u0 ^ rq, qh, ql);
+        uint32_t c0[V], c1[V], c2[V], c3[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            uint32_t hi;
+            mul_wide(kPhiloxM1, qh ^ a3[e], hi, c1[e]);
+            c0[e] = hi ^ b1[e];
+            c2[e] = r0h[e] ^ ql;
+            c3[e] = r0l[e];
+        }
+        uint32_t k0 = k.k0 + 3 * kPhiloxW0, k1 = k.k1 + 3 * kPhiloxW1;
+#pragma unroll
+        for (int r = 3; r < 10; ++r) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                uint32_t h0, l0, h1, l1;
+                mul_wide(kPhiloxM0, c0[e], h0, l0);
+                mul_wide(kPhiloxM1, c2[e], h1, l1);
+                asm("v_bitop3_b32 %0, %1, %2, %3 bitop3:0x96" : "=v"(c0[e]) : "v"(h1), "v"(c1[e]), "s"(k0));
+                asm("v_bitop3_b32 %0, %1, %2, %3 bitop3:0x96" : "=v"(c2[e]) : "v"(h0), "v"(c3[e]), "s"(k1));
+                c1[e] = l1;
+                c3[e] = l0;
+            }
+            k0 += kPhiloxW0;
+            k1 += kPhiloxW1;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            kept[0][e] = c0[e] < k.thr;
+            kept[1][e] = c1[e] < k.thr;
+            kept[2][e] = c2[e] < k.thr;
+            kept[3][e] = c3[e] < k.thr;
+        }
+    }
+};
+
+// A quad's mask as a word, and back.
+template <int V>
+__device__ __forceinline__ uint32_t pack_kept(const bool (&kept)[4][V]) {
     uint32_t bits = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const U32x4 o = philox4x32_10(U32x4{col + e, rq, k.tag, k.counter}, k.k0, k.k1);
-        bits |= (o.x < k.thr ? 1u : 0u) << (4 * e);
-        bits |= (o.y < k.thr ? 2u : 0u) << (4 * e);
-        bits |= (o.z < k.thr ? 4u : 0u) << (4 * e);
-        bits |= (o.w < k.thr ? 8u : 0u) << (4 * e);
-    }
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) bits |= kept[r][e] ? 1u << (r * V + e) : 0u;
     return bits;
+}
+template <int V>
+__device__ __forceinline__ void unpack_kept(uint32_t bits, bool (&kept)[4][V]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) kept[r][e] = (bits >> (r * V + e)) & 1u;
 }
 
 // keep in [0, 1] -> the threshold; false when every element is kept.

@@ -329,8 +329,11 @@ def ptr(t) -> int:
     return t.data_ptr()
 
 
-def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def stream_of(device) -> int:
+    """The current stream of a device (torch.device or index) as a hipStream_t."""
+    index = device if isinstance(device, int) else device.index
+    # the handle itself (0.1 us on the host); current_stream() builds a Stream object (2 us)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

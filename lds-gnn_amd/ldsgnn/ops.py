@@ -402,11 +402,12 @@ def aggregate(z: torch.Tensor, graph: CsrGraph) -> torch.Tensor:
 def _call_on(t: torch.Tensor, name: str, *args) -> None:
     """One entry point on `t`'s device, on that device's current stream (its
     last argument), whatever the current device is."""
-    if t.device.index == torch.cuda.current_device():
-        nat.call(name, *args, nat.stream_of(t.device))
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        nat.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(t.device):
-            nat.call(name, *args, nat.stream_of(t.device))
+        with torch.cuda.device(index):
+            nat.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _element_code(t: torch.Tensor, what: str) -> int:

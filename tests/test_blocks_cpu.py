@@ -74,7 +74,7 @@ def _norm(back=False, **kw):
 
 
 @pytest.mark.parametrize("back", [False, True])
-@pytest.mark.parametrize("kw", [dict(x=0), dict(y=0), dict(mean=0), dict(rstd=0), dict(ws=0), dict(ldx=7),
+@pytest.mark.parametrize("kw", [dict(x=0), dict(y=0), dict(mean=0), dict(rstd=0), dict(ws=0, n=200000), dict(ldx=7),
                                 dict(groups=3), dict(groups=0), dict(groups=-2), dict(dtype=3), dict(act=3),
                                 dict(act=-1), dict(pt=5), dict(keep=-1.0), dict(keep=float("nan")), dict(n=-1),
                                 dict(samples=-1), dict(c=-8), dict(samples=1 << 16, n=1 << 16), dict(sx=-1)])
@@ -90,9 +90,11 @@ def test_group_norm_workspace_sizes():
     size = nat.lib.lds_group_norm_ws_bytes
     assert size(1, 0, 8, 2, 0, 0) == 0 and size(0, 8, 8, 2, 0, 1) == 0
     assert size(1, 8, 8, 3, 0, 0) == -1 and size(1, 8, 8, 2, 7, 0) == -1 and size(-1, 8, 8, 2, 0, 0) == -1
-    for s, n, c, g in ((1, 1, 8, 2), (16, 2708, 60, 12), (8, 20000, 256, 32), (1, 3, 2051, 1)):
-        for dt in (0, 1, 2):
-            assert size(s, n, c, g, dt, 0) > 0 and size(s, n, c, g, dt, 1) > 0
+    for dt in (0, 1, 2):
+        # rows that a block holds need no workspace; longer ones do
+        assert size(1, 1, 8, 2, dt, 0) == 0 and size(1, 1, 8, 2, dt, 1) == 0
+        assert size(2, 1, 8, 2, dt, 1) == 2 * 8 * 8
+        assert size(8, 20000, 256, 32, dt, 0) > 0 and size(8, 20000, 256, 32, dt, 1) > 0
 
 
 def _quant(**kw):

@@ -166,6 +166,7 @@ def norm_bounds(x64, groups, w, b, eps):
 NORM_SHAPES = [  # samples, n, groups, channels per group
     (1, 1, 1, 1), (1, 1, 32, 8), (3, 1, 2, 3), (2, 7, 4, 5), (1, 5, 1, 2), (5, 33, 3, 16), (2, 100, 1, 700),
     (1, 9, 2, 4096), (1, 3, 1, 2051), (4, 515, 12, 5), (1, 2708, 4, 4), (2, 600, 32, 8), (17, 2, 300, 2),
+    (9, 1501, 3, 7), (1, 9001, 2, 4), (2, 5003, 2, 16), (1, 40, 1, 8200),
 ]
 
 
