@@ -108,6 +108,18 @@ struct Quad {
     }
 };
 
+// f(q, rows) for a thread's quads of a part: whole quads (all but a sample's
+// first and last) with the row limits as constants.
+template <typename F>
+__device__ __forceinline__ void each_quad(const NormArgs& a, const NormPlace& p, F&& f) {
+    for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
+        if (4 * q >= p.f0 && 4 * q + 4 <= p.f1)
+            f(q, QuadRows{0, 4});
+        else
+            f(q, quad_rows(p, q));
+    }
+}
+
 template <typename F>
 __device__ __forceinline__ F lane_xor(F v, int o) {
     return __shfl_xor(v, o);
@@ -117,16 +129,26 @@ __device__ __forceinline__ float2 lane_xor<float2>(float2 v, int o) {
     return make_float2(__shfl_xor(v.x, o), __shfl_xor(v.y, o));
 }
 
-// Σ over each group of the chunk of a value per thread, in a fixed order; every
-// thread gets its own group's sum.  red: one value per thread, then one per
-// group behind them.
+// Σ over each group of the chunk of a value per thread (0 where the thread has
+// none), in a fixed order; every thread gets its own group's sum.  red: a value
+// per thread, then one per group.  Two sums in a row need no barrier between
+// them if they use different `red`.
 template <typename F, int NT>
 __device__ __forceinline__ F group_sum(F v, const NormArgs& a, const NormPlace& p, F* red, int threads) {
     const int per = a.sub == 1 ? a.lanes / a.lpg : 1;
+    if (per == 1) {  // one group: the whole block
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) v += lane_xor(v, o);
+        if (threads == kWave) return v;
+        if (wave_lane() == 0) red[wave_id()] = v;
+        __syncthreads();
+        F sum = red[0];
+        for (int w = 1; w < threads / kWave; ++w) sum += red[w];
+        return sum;
+    }
     const int members = a.ty * a.lpg;
     int team = kWave;  // lanes per group: a power of two, no more than there are members
     while (team > 1 && team / 2 >= members) team /= 2;
-    __syncthreads();
     red[threadIdx.x] = v;
     __syncthreads();
     const int lane = threadIdx.x & (team - 1);
@@ -140,8 +162,7 @@ __device__ __forceinline__ F group_sum(F v, const NormArgs& a, const NormPlace& 
         if (lane == 0) red[NT + g] = sum;
     }
     __syncthreads();
-    const int g = a.sub == 1 ? p.tx / a.lpg : 0;
-    return red[NT + g];
+    return red[NT + (a.sub == 1 ? p.tx / a.lpg : 0)];
 }
 
 // The masks of a slab thread's Q quads, drawn before the rows are loaded: the
@@ -175,31 +196,37 @@ template <int ACT>
 __device__ __forceinline__ float act_grad(float z) {
     if constexpr (ACT == LDS_ACT_RELU) return z <= 0.f ? 0.f : 1.f;
     if constexpr (ACT == LDS_ACT_SILU) {
-        const float s = sigmoid_f(z);
-        return s * (1.f + z * (1.f - s));
+        const float s = sigmoid_f(z);  // s + z s (1 - s)
+        return __builtin_fmaf(s, __builtin_fmaf(-z, s, z), s);
     }
     return 1.f;
 }
 
-// γ, β of a thread's channels.
+// γ rstd and β of a thread's channels: z = (x - mean) (γ rstd) + β.
 template <int V>
 struct NormParams {
-    float w[V], b[V];
+    float rw[V], b[V];
 
+    static __device__ __forceinline__ void values(const void* p, int code, int c0, float (&f)[V]) {
+        if (code == LDS_F32)
+            load_vec<float, V>(reinterpret_cast<const float*>(p) + c0, f);
+        else if (code == LDS_BF16)
+            load_vec<bf16_t, V>(reinterpret_cast<const bf16_t*>(p) + c0, f);
+        else
+            load_vec<f16_t, V>(reinterpret_cast<const f16_t*>(p) + c0, f);
+    }
     __device__ __forceinline__ void load(const NormArgs& a, int c0) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            w[e] = 1.f;
+            rw[e] = 1.f;
             b[e] = 0.f;
         }
-        if (a.weight) {
+        if (a.weight) values(a.weight, a.ptype, c0, rw);
+        if (a.bias) values(a.bias, a.ptype, c0, b);
+    }
+    __device__ __forceinline__ void times(float rs) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = load_param(a.weight, a.ptype, c0 + e);
-        }
-        if (a.bias) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) b[e] = load_param(a.bias, a.ptype, c0 + e);
-        }
+        for (int e = 0; e < V; ++e) rw[e] *= rs;
     }
 };
 

@@ -8,28 +8,29 @@
 
 namespace lds {
 
-// x̂ and h of a quad.
+// x - mean and h / scale of a quad.
 template <typename T, int V, int ACT, bool DROP>
 struct BackQuad {
-    float xh[4][V], h[4][V];
+    float d[4][V], h[4][V];
 
     __device__ __forceinline__ void eval(const Quad<T, V>& x, const Quad<T, V>& g, const NormParams<V>& par, float mu,
-                                         float rs, const bool (&kept)[4][V], float scale) {
+                                         const bool (&kept)[4][V]) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                xh[r][e] = (elem<T, V>(x.row[r], e) - mu) * rs;
-                float d = elem<T, V>(g.row[r], e);
-                if constexpr (DROP) d = kept[r][e] ? d * scale : 0.f;
+                d[r][e] = elem<T, V>(x.row[r], e) - mu;
+                float t = elem<T, V>(g.row[r], e);
+                if constexpr (DROP) t = kept[r][e] ? t : 0.f;
                 if constexpr (ACT == LDS_ACT_RELU) {
-                    d = __builtin_fmaf(xh[r][e], par.w[e], par.b[e]) <= 0.f ? 0.f : d;
+                    t = __builtin_fmaf(d[r][e], par.rw[e], par.b[e]) <= 0.f ? 0.f : t;
                 } else if constexpr (ACT != LDS_ACT_NONE) {
-                    d *= act_grad<ACT>(__builtin_fmaf(xh[r][e], par.w[e], par.b[e]));
+                    t *= act_grad<ACT>(__builtin_fmaf(d[r][e], par.rw[e], par.b[e]));
                 }
-                h[r][e] = d;
+                h[r][e] = t;
             }
     }
+    // Σ h and Σ h (x - mean), both over scale
     __device__ __forceinline__ void sums(const QuadRows& in, float (&sh)[V], float (&sx)[V]) const {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -37,22 +38,33 @@ struct BackQuad {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 sh[e] += h[r][e];
-                sx[e] = __builtin_fmaf(h[r][e], xh[r][e], sx[e]);
+                sx[e] = __builtin_fmaf(h[r][e], d[r][e], sx[e]);
             }
         }
     }
-    __device__ __forceinline__ void store(const QuadRows& in, const NormParams<V>& par, float rs, float m1, float m2,
+    // dx = (γ rstd scale) h + (-(rstd² m2) (x - mean) - rstd m1)
+    __device__ __forceinline__ void store(const QuadRows& in, const float (&rws)[V], float k0, float k1,
                                           T* __restrict__ at, int64_t ld) const {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (r < in.lo || r >= in.hi) continue;
             float o[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = rs * (__builtin_fmaf(par.w[e], h[r][e], -m1) - xh[r][e] * m2);
+            for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(rws[e], h[r][e], __builtin_fmaf(k1, d[r][e], k0));
             store_vec<T, V>(at + r * ld, o);
         }
     }
 };
+
+// A thread's channel sums from those of BackQuad::sums.
+template <int V>
+__device__ __forceinline__ void finish_sums(float (&sh)[V], float (&sx)[V], float scale, float rs) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        sh[e] *= scale;
+        sx[e] *= scale * rs;
+    }
+}
 
 // The two sums of every channel of a block's chunk over its ty rows: value
 // i of a thread at red[i][thread], V values at a time.  Channel i of the chunk
@@ -123,11 +135,13 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
     }
     float mu = 0.f, rs = 0.f;
     NormParams<V> par{};
+    const float scale = DROP ? a.key.scale : 1.f;
     float sh[V] = {}, sx[V] = {};
     if (p.live) {
         mu = mean[s * a.groups + p.group];
         rs = rstd[s * a.groups + p.group];
         par.load(a, p.c0);
+        par.times(rs);
     }
     BackQuad<T, V, ACT, DROP> b;
 #pragma unroll
@@ -136,9 +150,10 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
         if (!p.live || q >= p.q1) continue;
         bool kept[4][V];
         if constexpr (DROP) unpack_kept<V>(masks[k], kept);
-        b.eval(v[k], g[k], par, mu, rs, kept, a.key.scale);
+        b.eval(v[k], g[k], par, mu, kept);
         b.sums(quad_rows(p, q), sh, sx);
     }
+    finish_sums<V>(sh, sx, scale, rs);
     if (sums || dweight || dbias) {
         const int c0 = chunk_first(a, chunk, V), c1 = chunk_last(a, chunk);
         channel_sums<V, NT>(sh, sx, a, chan, blockDim.x, [&](int i, float h, float hx) {
@@ -155,13 +170,15 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
     float2 m = make_float2(0.f, 0.f);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        m.x = __builtin_fmaf(par.w[e], sh[e], m.x);
-        m.y = __builtin_fmaf(par.w[e], sx[e], m.y);
+        m.x = __builtin_fmaf(par.rw[e], sh[e], m.x);
+        m.y = __builtin_fmaf(par.rw[e], sx[e], m.y);
     }
     m = group_sum<float2, NT>(m, a, p, red, blockDim.x);
     const float inv = 1.f / ((float)a.n * (float)a.cg);
-    const float m1 = m.x * inv, m2 = m.y * inv;
     if (!p.live) return;
+    const float k0 = -m.x * inv, k1 = -rs * (m.y * inv);  // of γ rstd: one rstd is in the sums
+#pragma unroll
+    for (int e = 0; e < V; ++e) par.rw[e] *= Q > 1 ? 1.f : scale;
     T* ds = dx + p.c0;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -170,9 +187,12 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
         if constexpr (Q > 1) {
             bool kept[4][V];
             if constexpr (DROP) unpack_kept<V>(masks[k], kept);
-            b.eval(v[k], g[k], par, mu, rs, kept, a.key.scale);
+            b.eval(v[k], g[k], par, mu, kept);
         }
-        b.store(quad_rows(p, q), par, rs, m1, m2, ds + 4 * q * a.c, a.c);
+        float rws[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) rws[e] = Q > 1 ? par.rw[e] * scale : par.rw[e];
+        b.store(quad_rows(p, q), rws, k0, k1, ds + 4 * q * a.c, a.c);
     }
 }
 
@@ -197,17 +217,18 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __re
         if constexpr (DROP) columns.init(a.key, (uint32_t)p.c0);
         const T* xs = x + p.s * a.sx + p.c0;
         const T* gs = dy + p.s * sdy + p.c0;
-        for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
-            const QuadRows in = quad_rows(p, q);
+        par.times(rs);
+        each_quad(a, p, [&](int64_t q, const QuadRows in) {
             Quad<T, V> v, g;
             v.load(xs, a.ldx, p, q, in);
             g.load(gs, lddy, p, q, in);
-            BackQuad<T, V, ACT, DROP> b;
             bool kept[4][V];
             if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-            b.eval(v, g, par, mu, rs, kept, a.key.scale);
+            BackQuad<T, V, ACT, DROP> b;
+            b.eval(v, g, par, mu, kept);
             b.sums(in, sh, sx);
-        }
+        });
+        finish_sums<V>(sh, sx, DROP ? a.key.scale : 1.f, rs);
     }
     const int c0 = chunk_first(a, p.chunk, V), c1 = chunk_last(a, p.chunk);
     channel_sums<V, kNormThreads>(sh, sx, a, red, kNormThreads, [&](int i, float h, float hx) {
@@ -294,17 +315,21 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
     const T* xs = x + p.s * a.sx + p.c0;
     const T* gs = dy + p.s * sdy + p.c0;
     T* ds = dx + p.c0;
-    for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
-        const QuadRows in = quad_rows(p, q);
+    par.times(rs);
+    float rws[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) rws[e] = DROP ? par.rw[e] * a.key.scale : par.rw[e];
+    const float k0 = -rs * m.x, k1 = -rs * rs * m.y;
+    each_quad(a, p, [&](int64_t q, const QuadRows in) {
         Quad<T, V> v, g;
         v.load(xs, a.ldx, p, q, in);
         g.load(gs, lddy, p, q, in);
-        BackQuad<T, V, ACT, DROP> b;
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-        b.eval(v, g, par, mu, rs, kept, a.key.scale);
-        b.store(in, par, rs, m.x, m.y, ds + 4 * q * a.c, a.c);
-    }
+        BackQuad<T, V, ACT, DROP> b;
+        b.eval(v, g, par, mu, kept);
+        b.store(in, rws, k0, k1, ds + 4 * q * a.c, a.c);
+    });
 }
 
 }  // namespace lds

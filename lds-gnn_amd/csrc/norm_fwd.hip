@@ -9,10 +9,10 @@ struct Moments {
     float count, m2;
 };
 
-// y of a quad from x: z = ((x - mean) rstd) γ + β.
+// y of a quad from x.
 template <typename T, int V, int ACT, bool DROP>
 __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& in, const NormParams<V>& par, float mu,
-                                           float rs, const bool (&kept)[4][V], float scale, T* __restrict__ at,
+                                           const bool (&kept)[4][V], float scale, T* __restrict__ at,
                                            int64_t ld) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -20,7 +20,7 @@ __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& 
         float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float z = __builtin_fmaf((elem<T, V>(x.row[r], e) - mu) * rs, par.w[e], par.b[e]);
+            const float z = __builtin_fmaf(elem<T, V>(x.row[r], e) - mu, par.rw[e], par.b[e]);
             o[e] = act_f<ACT>(z);
             if constexpr (DROP) o[e] = kept[r][e] ? o[e] * scale : 0.f;
         }
@@ -36,7 +36,7 @@ template <typename T, int V, int ACT, bool DROP, int Q>
 __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, NormArgs a, float eps,
                                                        T* __restrict__ y, float* __restrict__ mean,
                                                        float* __restrict__ rstd) {
-    __shared__ float2 red[2 * 1024];
+    __shared__ float2 red[2][2 * 1024];
     int64_t s;
     int chunk;
     if (!slab_place(a, s, chunk)) return;
@@ -54,6 +54,8 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, 
     // the data costs no digits; then, about that mean, the squares and what
     // the mean is still off by (the first value may be an outlier).
     const float first = p.live ? (float)x[s * a.sx + (int64_t)p.group * a.cg] : 0.f;
+    NormParams<V> par;
+    if (p.live) par.load(a, p.c0);
     const float inv = 1.f / ((float)a.n * (float)a.cg);
     float sum = 0.f;
 #pragma unroll
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, 
                 for (int e = 0; e < V; ++e) sum += elem<T, V>(v[k].row[r], e) - first;
             }
     }
-    const float m0 = first + group_sum<float, 1024>(sum, a, p, (float*)red, blockDim.x) * inv;
+    const float m0 = first + group_sum<float, 1024>(sum, a, p, (float*)red[0], blockDim.x) * inv;
     float2 d2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -86,16 +88,15 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, 
                 }
             }
     }
-    d2 = group_sum<float2, 1024>(d2, a, p, red, blockDim.x);
+    d2 = group_sum<float2, 1024>(d2, a, p, red[1], blockDim.x);
     const float off = d2.x * inv, mu = m0 + off;
     const float rs = 1.f / sqrtf(fmaxf(__builtin_fmaf(-off, off, d2.y * inv), 0.f) + eps);
     if (!p.live) return;
+    par.times(rs);
     if (p.ty == 0 && p.c0 == p.group * a.cg) {
         mean[s * a.groups + p.group] = mu;
         rstd[s * a.groups + p.group] = rs;
     }
-    NormParams<V> par;
-    par.load(a, p.c0);
     T* ys = y + p.c0;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, 
         if (q >= p.q1) continue;
         bool kept[4][V];
         if constexpr (DROP) unpack_kept<V>(masks[k], kept);
-        apply_quad<T, V, ACT, DROP>(v[k], quad_rows(p, q), par, mu, rs, kept, a.key.scale, ys + 4 * q * a.c, a.c);
+        apply_quad<T, V, ACT, DROP>(v[k], quad_rows(p, q), par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c);
     }
 }
 
@@ -157,25 +158,23 @@ __device__ __forceinline__ void quad_moments(const Quad<T, V>& v, const QuadRows
 template <typename T, int V>
 __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const T* __restrict__ x, NormArgs a,
                                                                 Moments* __restrict__ out) {
-    __shared__ double red[2 * kNormThreads];
+    __shared__ double red[3][2 * kNormThreads];
     const NormPlace p = norm_part_place(a, V);
     double mean = 0.0;
     float m2 = 0.f, cnt = 0.f;
     if (p.live) {
         const T* xs = x + p.s * a.sx + p.c0;
-#pragma unroll 2
-        for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
-            const QuadRows in = quad_rows(p, q);
+        each_quad(a, p, [&](int64_t q, const QuadRows in) {
             Quad<T, V> v;
             v.load(xs, a.ldx, p, q, in);
             quad_moments<T, V>(v, in, mean, m2, cnt);
-        }
+        });
     }
-    const double c = group_sum<double, kNormThreads>((double)cnt, a, p, red, kNormThreads);
+    const double c = group_sum<double, kNormThreads>((double)cnt, a, p, red[0], kNormThreads);
     const double gm =
-        group_sum<double, kNormThreads>((double)cnt * mean, a, p, red, kNormThreads) / (c > 0.0 ? c : 1.0);
+        group_sum<double, kNormThreads>((double)cnt * mean, a, p, red[1], kNormThreads) / (c > 0.0 ? c : 1.0);
     const float d = (float)(mean - gm);
-    const double g2 = group_sum<double, kNormThreads>(cnt > 0.f ? (double)(m2 + cnt * d * d) : 0.0, a, p, red,
+    const double g2 = group_sum<double, kNormThreads>(cnt > 0.f ? (double)(m2 + cnt * d * d) : 0.0, a, p, red[2],
                                                       kNormThreads);
     const int at = a.sub == 1 ? 0 : p.chunk - p.group * a.sub;
     if (p.live && p.ty == 0 && (a.sub == 1 ? p.tx % a.lpg == 0 : p.tx == 0))
@@ -226,14 +225,14 @@ __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restr
     if constexpr (DROP) columns.init(a.key, (uint32_t)p.c0);
     const T* xs = x + p.s * a.sx + p.c0;
     T* ys = y + p.c0;
-    for (int64_t q = p.q0 + p.ty; q < p.q1; q += a.ty) {
-        const QuadRows in = quad_rows(p, q);
+    par.times(rs);
+    each_quad(a, p, [&](int64_t q, const QuadRows in) {
         Quad<T, V> v;
         v.load(xs, a.ldx, p, q, in);
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-        apply_quad<T, V, ACT, DROP>(v, in, par, mu, rs, kept, a.key.scale, ys + 4 * q * a.c, a.c);
-    }
+        apply_quad<T, V, ACT, DROP>(v, in, par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c);
+    });
 }
 
 }  // namespace lds
