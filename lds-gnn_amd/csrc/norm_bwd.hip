@@ -56,6 +56,11 @@ struct BackQuad {
     }
 };
 
+template <typename T, int V>
+struct QuadPair {
+    Quad<T, V> x, g;
+};
+
 // A thread's channel sums from those of BackQuad::sums.
 template <int V>
 __device__ __forceinline__ void finish_sums(float (&sh)[V], float (&sx)[V], float scale, float rs) {
@@ -218,14 +223,17 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __re
         const T* xs = x + p.s * a.sx + p.c0;
         const T* gs = dy + p.s * sdy + p.c0;
         par.times(rs);
-        each_quad(a, p, [&](int64_t q, const QuadRows in) {
-            Quad<T, V> v, g;
-            v.load(xs, a.ldx, p, q, in);
-            g.load(gs, lddy, p, q, in);
+        each_quad_ahead<QuadPair<T, V>>(
+            a, p,
+            [&](QuadPair<T, V>& d, int64_t q, const QuadRows in) {
+                d.x.load(xs, a.ldx, p, q, in);
+                d.g.load(gs, lddy, p, q, in);
+            },
+            [&](const QuadPair<T, V>& d, int64_t q, const QuadRows in) {
             bool kept[4][V];
             if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
             BackQuad<T, V, ACT, DROP> b;
-            b.eval(v, g, par, mu, kept);
+            b.eval(d.x, d.g, par, mu, kept);
             b.sums(in, sh, sx);
         });
         finish_sums<V>(sh, sx, DROP ? a.key.scale : 1.f, rs);
@@ -320,14 +328,17 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
 #pragma unroll
     for (int e = 0; e < V; ++e) rws[e] = DROP ? par.rw[e] * a.key.scale : par.rw[e];
     const float k0 = -rs * m.x, k1 = -rs * rs * m.y;
-    each_quad(a, p, [&](int64_t q, const QuadRows in) {
-        Quad<T, V> v, g;
-        v.load(xs, a.ldx, p, q, in);
-        g.load(gs, lddy, p, q, in);
+    each_quad_ahead<QuadPair<T, V>>(
+        a, p,
+        [&](QuadPair<T, V>& d, int64_t q, const QuadRows in) {
+            d.x.load(xs, a.ldx, p, q, in);
+            d.g.load(gs, lddy, p, q, in);
+        },
+        [&](const QuadPair<T, V>& d, int64_t q, const QuadRows in) {
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
         BackQuad<T, V, ACT, DROP> b;
-        b.eval(v, g, par, mu, kept);
+        b.eval(d.x, d.g, par, mu, kept);
         b.store(in, rws, k0, k1, ds + 4 * q * a.c, a.c);
     });
 }

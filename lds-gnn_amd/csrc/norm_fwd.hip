@@ -266,9 +266,16 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     a.weight = weight;
     a.bias = bias;
     a.ptype = ptype;
+    NormArgs b = a;  // the second pass of the parts form
+    if (!k.slab) {
+        const NormArgs cut = norm_plan(samples, n, c, groups, dtype, kForwardSlabThreads, kApplyBlocks).a;
+        b.parts = cut.parts;
+        b.part_q = cut.part_q;
+    }
     const int64_t blocks = k.slab ? slab_blocks(a) : samples * a.parts * a.chunks;
     const int64_t pairs = samples * groups;
-    LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && pairs < (int64_t)1 << 32);
+    LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && samples * b.parts * b.chunks < (int64_t)1 << 31);
+    LDS_CHECK_ARG(pairs < (int64_t)1 << 32);
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
         return with_vec<16 / (int)sizeof(T)>(k.v, [&](auto vc) -> int {
@@ -289,8 +296,9 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
                                            mean, rstd);
                     };
                     if (!k.slab)
-                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
-                                           dim3(kNormThreads), 0, st, (const T*)x, a, mean, rstd, (T*)y);
+                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>),
+                                           dim3((unsigned)(samples * b.parts * b.chunks)), dim3(kNormThreads), 0, st,
+                                           (const T*)x, b, mean, rstd, (T*)y);
                     else if (k.quads == 1)
                         slab(IntC<1>{});
                     else if (k.quads == 2)
