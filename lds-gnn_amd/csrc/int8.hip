@@ -508,3 +508,17 @@ extern "C" int lds_int8_matmul(const signed char* xq, int64_t ldx, const float* 
         return launch_split<T, 4, 2, 8>(a, (T*)y, st);
     });
 }
+
+extern "C" int lds_int8_linear(const void* x, int64_t ldx, int xdtype, signed char* q, int64_t ldq, float* xs,
+                               const signed char* wq, int64_t ldw, const float* ws, const void* bias, int ptype,
+                               int64_t m, int n, int k, void* y, int64_t ldy, int dtype, void* stream) {
+    // the product's checks come first: nothing is launched by a refused call
+    LDS_CHECK_ARG(m >= 0 && m <= (int64_t)0x7fffffff && n >= 0 && k >= 0 && k <= 131071);
+    LDS_CHECK_ARG(dtype >= LDS_F32 && dtype <= LDS_F16 && ptype >= LDS_F32 && ptype <= LDS_F16);
+    if (m == 0 || n == 0) return 0;
+    LDS_CHECK_ARG(xs && ws && y && ldy >= n);
+    LDS_CHECK_ARG(k == 0 || (q && wq && ldq >= k && ldw >= k && ldq % 16 == 0 && ldw % 16 == 0 &&
+                             (((uintptr_t)q | (uintptr_t)wq) & 15) == 0));
+    const int e = lds_quantize_rows(x, ldx, m, k, xdtype, q, ldq, xs, stream);
+    return e ? e : lds_int8_matmul(q, ldq, xs, wq, ldw, ws, bias, ptype, m, n, k, y, ldy, dtype, stream);
+}

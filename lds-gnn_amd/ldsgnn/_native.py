@@ -95,6 +95,8 @@ SIGNATURES = {
                                 c_int, c_int, c_float, c_float, c_uint64, c_uint32, c_uint32, P, P, P, P, P, P, P],
     "lds_quantize_rows": [P, c_int64, c_int64, c_int, c_int, P, c_int64, P, P],
     "lds_int8_matmul": [P, c_int64, P, P, c_int64, P, P, c_int, c_int64, c_int, c_int, P, c_int64, c_int, P],
+    "lds_int8_linear": [P, c_int64, c_int, P, c_int64, P, P, c_int64, P, P, c_int, c_int64, c_int, c_int, P, c_int64,
+                        c_int, P],
     # fused engine (csrc/engine.hip)
     "lds_engine_scalars_size": [],
     "lds_sample_bitmask_dev": [P, c_int, c_uint64, c_uint32, P, c_uint32, P, c_int, P],

@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes
 from typing import List, Optional, Tuple
 
+import numpy as np
 import torch
 from torch.autograd import Function
 
@@ -424,9 +425,14 @@ def _rows_of(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     if t.dim() == 0:
         raise ValueError(f"ldsgnn {what}: expected at least one dimension")
     cols = t.size(-1)
-    if t.is_contiguous():
-        return t, (t.numel() // cols if cols else 0), cols, cols
-    rows = t.numel() // cols if cols else 0
+    if cols:
+        rows = t.numel() // cols
+    else:
+        rows = 1
+        for d in t.shape[:-1]:
+            rows *= d
+    if t.is_contiguous() or t.numel() == 0:
+        return t, rows, cols, cols
     try:
         v = t.view(rows, cols)
     except RuntimeError:
@@ -442,7 +448,8 @@ def _keep_scale(p: float, key, what: str) -> Tuple[float, float]:
         raise ValueError(f"ldsgnn {what}: p must lie in [0, 1], got {p}")
     if p > 0.0 and key is None:
         raise ValueError(f"ldsgnn {what}: dropout needs a key (seed, tag, counter)")
-    import numpy as np
+    if p == 0.0:
+        return 1.0, 1.0
     keep = np.float32(1.0) - np.float32(p)
     return float(keep), float(np.float32(1.0) / keep) if keep > 0 else 0.0
 
@@ -471,7 +478,7 @@ def _dropout_raw(x: torch.Tensor, keep: float, scale: float, key,
                  residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     code = _element_code(x, "dropout")
     xr, rows, cols, ldx = _rows_of(x, "dropout")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     rr, ldr = None, 0
     if residual is not None:
         rr, _, _, ldr = _rows_of(residual, "dropout residual")
@@ -541,17 +548,18 @@ def _norm_forward(x, weight, bias, pl: _NormPlan):
     xr, samples, n, sx, ldx = _samples_of(x)
     c = x.size(-1)
     dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=dev)
     stats = torch.empty((2, samples, pl.groups), dtype=torch.float32, device=dev)
     if x.numel() == 0:
         return y, stats
     pcode = 0 if weight is None and bias is None else nat.ELEMENT_CODES[(bias if weight is None else weight).dtype]
-    ws = torch.empty(nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 0), dtype=torch.uint8, device=dev)
+    size = nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 0)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     seed, tag, counter = pl.key if pl.key is not None else (0, 0, 0)
     at = stats.data_ptr()
     _call_on(x, "lds_group_norm_forward", xr.data_ptr(), sx, ldx, samples, n, c, pl.groups, code, nat.ptr(weight),
              nat.ptr(bias), pcode, pl.eps, pl.act, pl.keep, pl.scale, seed, tag, counter, y.data_ptr(), at,
-             at + 4 * samples * pl.groups, ws.data_ptr())
+             at + 4 * samples * pl.groups, nat.ptr(ws))
     return y, stats
 
 
@@ -564,18 +572,22 @@ def _norm_backward(gy, x, weight, bias, stats, pl: _NormPlan, need):
     want_w, want_b = need[1] and weight is not None, need[2] and bias is not None
     if x.numel() == 0:
         return (dx, torch.zeros_like(weight) if want_w else None, torch.zeros_like(bias) if want_b else None)
-    dpar = torch.empty((2, c), dtype=torch.float32, device=dev) if want_w or want_b else None
+    dw = torch.empty(c, dtype=torch.float32, device=dev) if want_w else None
+    db = torch.empty(c, dtype=torch.float32, device=dev) if want_b else None
     xr, samples, n, sx, ldx = _samples_of(x)
     gr, _, _, sg, ldg = _samples_of(gy)
     pcode = 0 if weight is None and bias is None else nat.ELEMENT_CODES[(bias if weight is None else weight).dtype]
-    ws = torch.empty(nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 1), dtype=torch.uint8, device=dev)
+    size = nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     seed, tag, counter = pl.key if pl.key is not None else (0, 0, 0)
-    at, dp = stats.data_ptr(), nat.ptr(dpar)
+    at = stats.data_ptr()
     _call_on(x, "lds_group_norm_backward", gr.data_ptr(), sg, ldg, xr.data_ptr(), sx, ldx, samples, n, c, pl.groups,
              code, nat.ptr(weight), nat.ptr(bias), pcode, pl.act, pl.keep, pl.scale, seed, tag, counter, at,
-             at + 4 * samples * pl.groups, nat.ptr(dx), dp if want_w else 0, dp + 4 * c if want_b else 0,
-             ws.data_ptr())
-    return (dx, dpar[0].to(weight.dtype) if want_w else None, dpar[1].to(bias.dtype) if want_b else None)
+             at + 4 * samples * pl.groups, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(ws))
+    if pcode:  # 16-bit parameters: one rounding of the fp32 sums
+        dw = dw if dw is None else dw.to(weight.dtype)
+        db = db if db is None else db.to(bias.dtype)
+    return dx, dw, db
 
 
 def _norm_composed(x, weight, bias, mask, pl: _NormPlan):
@@ -749,6 +761,29 @@ def _no_grad_only(what: str, *tensors) -> None:
         raise RuntimeError(f"ldsgnn {what}: the 8-bit product has no gradient; call it under torch.no_grad()")
 
 
+def _int8_weights(what: str, k: int, dev, wq, w_scale, bias, out_dtype):
+    """The checks of the weights' side; (wq, w_scale, bias, n, row stride, codes)."""
+    wq = _int8_readable(wq, what)
+    n, kw = wq.shape
+    code = nat.ELEMENT_CODES.get(out_dtype)
+    if code is None:
+        raise TypeError(f"ldsgnn {what}: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    if k != kw or k > INT8_MAX_K:
+        raise ValueError(f"ldsgnn {what}: inner sizes {k} and {kw} must agree and not exceed {INT8_MAX_K}")
+    if w_scale.shape != (n,) or w_scale.dtype != torch.float32 or w_scale.device != dev or wq.device != dev:
+        raise ValueError(f"ldsgnn {what}: wq and w_scale ({n} float32 values) must lie on {dev}, got "
+                         f"{tuple(w_scale.shape)}, {w_scale.dtype}, {w_scale.device}, {wq.device}")
+    pcode = 0
+    if bias is not None:
+        pcode = nat.ELEMENT_CODES.get(bias.dtype)
+        if bias.shape != (n,) or bias.device != dev or pcode is None:
+            raise ValueError(f"ldsgnn {what}: bias must hold {n} floating values on {dev}, got "
+                             f"{tuple(bias.shape)}, {bias.dtype}, {bias.device}")
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+    ldw = wq.stride(0) if n > 1 and k > 0 else _int8_stride(k)
+    return wq, (w_scale if w_scale.is_contiguous() else w_scale.contiguous()), bias, n, ldw, pcode, code
+
+
 def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """y = (xq wqᵀ) · x_scale per row · w_scale per output channel + bias
@@ -757,46 +792,41 @@ def int8_matmul(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_sca
     float16, rounded once.  Rows that do not start at multiples of 16 bytes are
     copied (int8_rows lays them out once).  No gradient."""
     _no_grad_only("int8_matmul", x_scale, w_scale, bias)
-    if out_dtype not in nat.ELEMENT_CODES:
-        raise TypeError(f"ldsgnn int8_matmul: out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
-    xq, wq = _int8_readable(xq, "int8_matmul"), _int8_readable(wq, "int8_matmul")
-    (m, k), (n, kw) = xq.shape, wq.shape
+    xq = _int8_readable(xq, "int8_matmul")
+    m, k = xq.shape
     dev = xq.device
-    if k != kw or k > INT8_MAX_K:
-        raise ValueError(f"ldsgnn int8_matmul: inner sizes {k} and {kw} must agree and not exceed {INT8_MAX_K}")
-    for name, t, size in (("x_scale", x_scale, m), ("w_scale", w_scale, n)):
-        if t.shape != (size,) or t.dtype != torch.float32 or t.device != dev:
-            raise ValueError(f"ldsgnn int8_matmul: {name} must be {size} float32 values on {dev}, got "
-                             f"{tuple(t.shape)}, {t.dtype}, {t.device}")
-    if wq.device != dev or (bias is not None and (bias.shape != (n,) or bias.device != dev or
-                                                  bias.dtype not in nat.ELEMENT_CODES)):
-        raise ValueError(f"ldsgnn int8_matmul: wq and bias ({n} floating values) must lie on {dev}")
-    x_scale, w_scale = x_scale.contiguous(), w_scale.contiguous()
-    bias = bias if bias is None else bias.contiguous()
+    if x_scale.shape != (m,) or x_scale.dtype != torch.float32 or x_scale.device != dev:
+        raise ValueError(f"ldsgnn int8_matmul: x_scale must be {m} float32 values on {dev}, got "
+                         f"{tuple(x_scale.shape)}, {x_scale.dtype}, {x_scale.device}")
+    wq, w_scale, bias, n, ldw, pcode, code = _int8_weights("int8_matmul", k, dev, wq, w_scale, bias, out_dtype)
+    x_scale = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
     y = torch.empty((m, n), dtype=out_dtype, device=dev)
-    wide = -(-k // 16) * 16
-    _call_on(xq, "lds_int8_matmul", xq.data_ptr(), xq.stride(0) if m > 1 and k > 0 else wide, x_scale.data_ptr(),
-             wq.data_ptr(), wq.stride(0) if n > 1 and k > 0 else wide, w_scale.data_ptr(), nat.ptr(bias),
-             0 if bias is None else nat.ELEMENT_CODES[bias.dtype], m, n, k, y.data_ptr(), n,
-             nat.ELEMENT_CODES[out_dtype])
+    _call_on(xq, "lds_int8_matmul", xq.data_ptr(), xq.stride(0) if m > 1 and k > 0 else _int8_stride(k),
+             x_scale.data_ptr(), wq.data_ptr(), ldw, w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), pcode,
+             m, n, k, y.data_ptr(), n, code)
     return y
 
 
 def int8_linear(x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """x (..., k) times an 8-bit weight: the rows of x are quantised
-    (quantize_rows) and multiplied (int8_matmul).  Result (..., n) in x's dtype
-    unless out_dtype names another.  No gradient."""
+    """x (..., k) times an 8-bit weight (lds_int8_linear): the rows of x are
+    quantised as quantize_rows does and multiplied as int8_matmul does.  Result
+    (..., n) in x's dtype unless out_dtype names another.  No gradient."""
     _no_grad_only("int8_linear", x, w_scale, bias)
-    _element_code(x, "int8_linear")
+    xcode = _element_code(x, "int8_linear")
     if x.dim() < 1:
         raise ValueError("ldsgnn int8_linear: expected (..., k)")
-    rows = 1
-    for d in x.shape[:-1]:
-        rows *= d
-    q, scale = quantize_rows(x if x.dim() == 2 else x.reshape(rows, x.size(-1)))
-    y = int8_matmul(q, scale, wq, w_scale, bias, x.dtype if out_dtype is None else out_dtype)
-    return y if x.dim() == 2 else y.view(x.shape[:-1] + (y.size(1),))
+    xr, m, k, ldx = _rows_of(x, "int8_linear")
+    dev = x.device
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    wq, w_scale, bias, n, ldw, pcode, code = _int8_weights("int8_linear", k, dev, wq, w_scale, bias, out_dtype)
+    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    ldq = _int8_stride(k)
+    ws = torch.empty(m * (ldq + 4), dtype=torch.uint8, device=dev)  # the rows, then their scales
+    at = ws.data_ptr()
+    _call_on(x, "lds_int8_linear", xr.data_ptr(), ldx, xcode, at, ldq, at + m * ldq, wq.data_ptr(), ldw,
+             w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), pcode, m, n, k, y.data_ptr(), n, code)
+    return y
 
 
 # ---------------------------------------------------------------------------

@@ -120,3 +120,13 @@ def _mul(**kw):
                                 dict(k=-1), dict(m=-1), dict(n=-1), dict(dtype=3), dict(pt=9)])
 def test_int8_matmul_entry_refuses(kw):
     assert _mul(**kw) == 1
+
+
+@pytest.mark.parametrize("kw", [dict(x=0), dict(xq=0), dict(wq=0), dict(xs=0), dict(ws=0), dict(y=0), dict(ldq=20),
+                                dict(ldw=24), dict(ldx=16), dict(ldy=4), dict(xq=FAKE + 4), dict(k=131072),
+                                dict(m=-1), dict(xdt=3), dict(dtype=3), dict(pt=-1)])
+def test_int8_linear_entry_refuses(kw):
+    a = dict(x=FAKE, ldx=20, xdt=0, xq=FAKE, ldq=32, xs=FAKE, wq=FAKE, ldw=32, ws=FAKE, bias=0, pt=0, m=3, n=5, k=20,
+             y=FAKE, ldy=5, dtype=0)
+    a.update(kw)
+    assert nat.lib.lds_int8_linear(*a.values(), None) == 1

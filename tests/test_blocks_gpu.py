@@ -484,6 +484,11 @@ def test_int8_matmul_whole_numbers(device, ops, m, n, k):
     a, b = ints(g, m, k), ints(g, n, k)
     one = torch.ones(max(m, n), device=device)
     y = ops.int8_matmul(a.to(device), one[:m], b.to(device), one[:n])
+    a127 = a.clone()
+    a127[:, 0] = 127  # the scale of the same numbers as fp32 rows is 1: the joint call gives the same
+    with torch.no_grad():
+        y127 = ops.int8_linear(a127.float().to(device), b.to(device), one[:n])
+    assert torch.equal(y127.cpu(), (a127.double() @ b.double().t()).float())
     assert torch.equal(y.cpu(), (a.double() @ b.double().t()).float())
 
 
@@ -545,6 +550,9 @@ def test_int8_matmul_empty(device, ops, m, n, k):
     bias = torch.arange(n, device=device).float()
     y = ops.int8_matmul(q, torch.ones(m, device=device), w, torch.ones(n, device=device), bias)
     assert y.shape == (m, n) and torch.equal(y, bias.expand(m, n))
+    with torch.no_grad():
+        z = ops.int8_linear(torch.zeros(m, k, device=device), w, torch.ones(n, device=device), bias)
+    assert z.shape == (m, n) and torch.equal(z, bias.expand(m, n))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
