@@ -577,6 +577,9 @@ class LdsEngine:
                 flat[..., self.off_b1:self.off_b1 + c])
 
     def _write_params(self, flat: torch.Tensor, params) -> None:
+        if any(".norm." in name for name in params):
+            raise NotImplementedError("the fused engine implements the GCN without a norm layer "
+                                      "(MetaDenseGCN(norm_groups=0)); train a normalised one with the trainers")
         w0t, b0, w1, b1 = self._views(flat)
         with torch.no_grad():
             w0t.view(self.fin, HID).copy_(params["layer_in.fc.weight"].detach().t())

@@ -9,6 +9,10 @@ lds_dropout kernel.  A fixed symmetric 0/1 adjacency on the device (the
 dataset graph of BASELINE config 1) is converted once to that CSR form
 (`fixed_graph`); any other dense tensor graph keeps the reference semantics
 (normalize_adjacency_matrix + torch.mm) on its device.
+
+norm_groups > 0 puts a group norm between the two layers in place of the bare
+relu: drop(act(norm(.))) as one operator (ldsgnn.ops.group_norm_act), with the
+same dropout keys.
 """
 from __future__ import annotations
 
@@ -18,9 +22,9 @@ import torch
 import torch.nn.functional as F
 
 from .. import rng as _rng
-from ..ops import CsrGraph, csr_graph_from_dense, keyed_dropout
+from ..ops import CsrGraph, csr_graph_from_dense, group_norm_act, int8_linear, keyed_dropout, quantize_rows
 from ..utils.graph import normalize_adjacency_matrix
-from .layers import MetaDenseGraphConvolution
+from .layers import MetaDenseGraphConvolution, _aggregate
 from .meta import MetaModule, get_subdict
 
 _FIXED: list = []  # [(weakref to the adjacency, its version, CsrGraph | None)], most recent last
@@ -52,9 +56,10 @@ def fixed_graph(adj: torch.Tensor):
 class MetaDenseGCN(MetaModule):
 
     def __init__(self, in_features, hidden_features, out_features, dropout, normalize_adj: bool = True,
-                 generator: "_rng.Generator" = None):
+                 generator: "_rng.Generator" = None, norm_groups: int = 0, norm_act: str = "relu"):
         super().__init__()
-        self.layer_in = MetaDenseGraphConvolution(in_features, hidden_features)
+        self.layer_in = MetaDenseGraphConvolution(in_features, hidden_features, norm_groups=norm_groups,
+                                                  norm_act=norm_act)
         self.layer_out = MetaDenseGraphConvolution(hidden_features, out_features)
         self.dropout = dropout
         self.normalize_adj = normalize_adj
@@ -79,7 +84,7 @@ class MetaDenseGCN(MetaModule):
             return x
         return keyed_dropout(x, self.dropout, key)  # HIP kernel; raises for CPU tensors
 
-    def forward_to_last_layer(self, node_features, dense_adj, params=None, dropout_counter: int = None):
+    def _graph(self, dense_adj):
         if isinstance(dense_adj, CsrGraph):
             if not self.normalize_adj:
                 raise NotImplementedError("hot-path graphs are normalised by construction "
@@ -90,12 +95,68 @@ class MetaDenseGCN(MetaModule):
             # CSR graph; anything else keeps the reference's dense semantics
             graph = fixed_graph(dense_adj)
             dense_adj = graph if graph is not None else normalize_adjacency_matrix(dense_adj)
+        return dense_adj
+
+    def forward_to_last_layer(self, node_features, dense_adj, params=None, dropout_counter: int = None):
+        dense_adj = self._graph(dense_adj)
         kx, kh = self._dropout_keys(dropout_counter)
         embeddings = self._drop(node_features, kx)
-        embeddings = F.relu(self.layer_in(embeddings, dense_adj, params=get_subdict(params, "layer_in")))
-        embeddings = self._drop(embeddings, kh)
+        embeddings = self.layer_in(embeddings, dense_adj, params=get_subdict(params, "layer_in"))
+        if self.layer_in.norm is not None:
+            embeddings = self.layer_in.norm(embeddings, params=get_subdict(params, "layer_in.norm"),
+                                            p=0.0 if kh is None else self.dropout, key=kh)
+        else:
+            embeddings = self._drop(F.relu(embeddings), kh)
         return self.layer_out(embeddings, dense_adj, params=get_subdict(params, "layer_out"))
 
     def forward(self, node_features, dense_adj, params=None):
         embeddings = self.forward_to_last_layer(node_features, dense_adj, params=params)
         return F.log_softmax(embeddings, dim=1)
+
+
+class Int8DenseGCN(torch.nn.Module):
+    """A trained MetaDenseGCN for evaluation, its two dense products in 8-bit
+    integers (ldsgnn.ops.int8_linear): the weights are quantised once, a scale
+    per output channel, the node features and hidden rows at every call, a
+    scale per node.  Aggregation, norm, activation and log_softmax stay fp32,
+    so a product's relative error is that of 8 bits (about 2^-8 of the row's
+    largest value).  No dropout, no gradient.
+
+        model8 = Int8DenseGCN(model)              # or params=trainer.model_params
+        evaluate(model8, data, graph)
+    """
+
+    def __init__(self, model: MetaDenseGCN, params=None):
+        super().__init__()
+        params = dict(model.named_parameters()) if params is None else dict(params)
+        self.normalize_adj = model.normalize_adj
+        norm = model.layer_in.norm
+        self.norm = None if norm is None else (norm.groups, norm.act, norm.eps)
+        with torch.no_grad():
+            for name in ("layer_in", "layer_out"):
+                q, scale = quantize_rows(params[name + ".fc.weight"].detach())
+                bias = params.get(name + ".fc.bias")
+                self.register_buffer(name + "_q", q)
+                self.register_buffer(name + "_scale", scale)
+                self.register_buffer(name + "_bias", None if bias is None else bias.detach().clone())
+            for part in ("weight", "bias"):
+                t = None if norm is None else params["layer_in.norm." + part].detach().clone()
+                self.register_buffer("norm_" + part, t)
+
+    _graph = MetaDenseGCN._graph
+
+    @torch.no_grad()
+    def forward_to_last_layer(self, node_features, dense_adj):
+        graph = self._graph(dense_adj)
+        h = _aggregate(graph, int8_linear(node_features, self.layer_in_q, self.layer_in_scale, self.layer_in_bias))
+        if self.norm is not None:
+            groups, act, eps = self.norm
+            h = group_norm_act(h, groups, self.norm_weight, self.norm_bias, act=act, eps=eps)
+        else:
+            h = F.relu(h)
+        return _aggregate(graph, int8_linear(h, self.layer_out_q, self.layer_out_scale, self.layer_out_bias))
+
+    def forward(self, node_features, dense_adj, params=None):
+        if params is not None:
+            raise ValueError("Int8DenseGCN holds its own weights: quantise new ones with Int8DenseGCN(model, params)")
+        return F.log_softmax(self.forward_to_last_layer(node_features, dense_adj), dim=1)

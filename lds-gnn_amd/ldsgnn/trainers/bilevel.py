@@ -85,12 +85,13 @@ class BilevelProblemRunner:
                 sacred_runner(name, value, current_step)
         return metrics
 
-    def evaluate(self) -> Dict:
+    def evaluate(self, int8: bool = False) -> Dict:
+        """int8: the GCN's dense products in 8-bit integers."""
         assert self.gcn_params is not None and self.graph_state_dict is not None, \
             "Models need to be trained before evaluation."
         self.outer_trainer.model.load_state_dict(self.graph_state_dict)
         val, test = empirical_mean_loss(self.inner_trainer.model, graph_model=self.outer_trainer.model,
                                         n_samples=self.n_samples_empirical_mean, data=self.data,
-                                        model_parameters=self.gcn_params)
+                                        model_parameters=self.gcn_params, int8=int8)
         return {"loss.val.final": val.loss, "acc.val.final": val.acc,
                 "loss.test.final": test.loss, "acc.test.final": test.acc}

@@ -11,14 +11,21 @@ from torch.nn import functional as F
 from ..trainers import Metrics
 
 
+def _int8_form(model, params):
+    from ..models.gcn import Int8DenseGCN
+    return model if isinstance(model, Int8DenseGCN) else Int8DenseGCN(model, params)
+
+
 def accuracy(predictions: torch.Tensor, labels: torch.Tensor) -> float:
     """src/utils/evaluation.py:15-22"""
     return (torch.argmax(predictions, dim=-1) == labels).float().mean().item()
 
 
-def evaluate(model: torch.nn.Module, data, adj_matrix=None) -> Dict:
-    """src/utils/evaluation.py:25-48; `adj_matrix` may be a hot-path graph."""
+def evaluate(model: torch.nn.Module, data, adj_matrix=None, int8: bool = False) -> Dict:
+    """src/utils/evaluation.py:25-48; `adj_matrix` may be a hot-path graph.
+    int8: the GCN's dense products in 8-bit integers (Int8DenseGCN)."""
     model.eval()
+    model = _int8_form(model, None) if int8 else model
     with torch.no_grad():
         graph = adj_matrix if adj_matrix is not None else (
             data.graph if getattr(data, "graph", None) is not None else data.dense_adj)
@@ -32,12 +39,15 @@ def evaluate(model: torch.nn.Module, data, adj_matrix=None) -> Dict:
 
 
 def empirical_mean_loss(gcn, graph_model, n_samples: int, data,
-                        model_parameters: OrderedDict = None) -> Tuple[Metrics, Metrics]:
+                        model_parameters: OrderedDict = None, int8: bool = False) -> Tuple[Metrics, Metrics]:
     """src/utils/evaluation.py:51-84: mean NLL/accuracy over `n_samples` graphs
     drawn from the graph model, no grad.  Losses stay on device and are reduced
-    once (one host sync instead of 4·S)."""
+    once (one host sync instead of 4·S).  int8: the GCN's dense products in
+    8-bit integers, its weights quantised once for all graphs."""
     gcn.eval()
     graph_model.eval()
+    if int8:
+        gcn, model_parameters = _int8_form(gcn, model_parameters), None
     with torch.no_grad():
         vals = []
         for _ in range(n_samples):
