@@ -551,9 +551,10 @@ int lds_int8_matmul(const signed char* xq, int64_t ldx, const float* xs,
                     const signed char* wq, int64_t ldw, const float* ws,
                     const void* bias, int ptype, int64_t m, int n, int k,
                     void* y, int64_t ldy, int dtype, void* stream);
-/* Both in one call: the rows of x (m × k elements `xdtype`) quantised into q
- * (m rows of ldq bytes) and xs (m floats), the caller's workspace, and
- * multiplied.  Arguments as above. */
+/* Both in one call: the rows of x (m × k elements `xdtype`) quantised and
+ * multiplied, the same result.  q (m rows of ldq bytes) and xs (m floats) are
+ * the caller's workspace; what they hold afterwards is not specified (a few
+ * rows are quantised on chip).  Arguments as above. */
 int lds_int8_linear(const void* x, int64_t ldx, int xdtype, signed char* q,
                     int64_t ldq, float* xs, const signed char* wq, int64_t ldw,
                     const float* ws, const void* bias, int ptype, int64_t m,

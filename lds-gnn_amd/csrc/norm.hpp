@@ -23,7 +23,6 @@ constexpr int kNormThreads = 256;  // a block of the parts form
 // waves are light: 36.2 us at 4096 with dropout, 38.6 at 512.
 constexpr int kSumBlocks = 512;
 constexpr int kApplyBlocks = 4096;
-constexpr int kSlabQuads = 4;      // row quads that a slab thread holds at most
 constexpr int kForwardSlabThreads = 1024;
 constexpr int kBackwardSlabThreads = 512;  // x and dy: twice the registers a thread
 
@@ -200,9 +199,9 @@ __device__ __forceinline__ F group_sum(F v, const NormArgs& a, const NormPlace& 
     return red[NT + (a.sub == 1 ? p.tx / a.lpg : 0)];
 }
 
-// The masks of a slab thread's Q quads, drawn before the rows are loaded: the
-// column products of the generator and the rows together would not fit the
-// registers of a block of 1024 threads.
+// The masks of a slab thread's Q quads, drawn while its registers hold nothing
+// else: the generator's column products and the rows together would not leave
+// room for a block of 1024 threads.
 template <int V, int Q>
 __device__ __forceinline__ void slab_masks(const NormArgs& a, const NormPlace& p, uint32_t (&bits)[Q]) {
     ColumnKeep<V> columns;
@@ -282,6 +281,16 @@ inline int with_vec(int v, F&& f) {
     return f(IntC<1>{});
 }
 
+// ... for a slab thread's quads: at most 32 values of x are held.
+template <int V, typename F>
+inline void with_quads(int quads, F&& f) {
+    if constexpr (V <= 2)
+        if (quads == 4) return f(IntC<4>{});
+    if constexpr (V <= 4)
+        if (quads == 2) return f(IntC<2>{});
+    f(IntC<1>{});
+}
+
 // The sizes that both directions accept; false: hipErrorInvalidValue.
 inline bool norm_sizes_ok(int64_t samples, int64_t n, int c, int groups) {
     if (samples < 0 || n < 0 || c < 0 || groups < 1 || c % groups) return false;
@@ -296,7 +305,7 @@ struct NormPlan {
     int v;
     bool slab;
     int threads;   // slab: 64 .. slab_threads
-    int quads;     // slab: row quads per thread, 1, 2 or 4
+    int quads;     // slab: row quads per thread: 1, or 2 (V <= 4), or 4 (V <= 2)
     NormArgs a;
 };
 
@@ -315,7 +324,7 @@ inline NormPlan norm_plan(int64_t samples, int64_t n, int c, int groups, int dty
     k.v = 16 / elem;
     while (k.v > 1 && a.cg % k.v) k.v /= 2;
     const int lpg = a.cg / k.v;
-    const int64_t quads = n / 4 + 2;  // a sample's quads, its partial first and last one among them
+    const int64_t quads = (n + 2) / 4 + 1;  // a sample's quads at most, wherever its first row lies in one
     a.part_q = quads;
     a.parts = 1;
     a.sub = 1;
@@ -324,24 +333,34 @@ inline NormPlan norm_plan(int64_t samples, int64_t n, int c, int groups, int dty
         const int ty = threads / (per * lpg);
         return ty < 1 ? INT64_MAX : (quads + ty - 1) / ty;
     };
-    if (lpg <= slab_threads && held(slab_threads, 1) <= kSlabQuads) {
-        k.slab = true;
-        // as few groups a block as there are, for more blocks; more where a
-        // row's share would be under a 64-byte line and blocks abound
+    // The slab form, where one block's arithmetic is short beside the two launches
+    // it saves: a group of up to 32768 values of a sample (forward; half of
+    // that backward).  One sample of 4000 x 8 channels a group, bf16: 10.2 us
+    // against 13.2 in parts, backward 15.0 / 13.7; of 8000: 15.6 / 13.1.  And,
+    // where there are more blocks than two per CU, only with whole lines to
+    // read: 200 samples of 2000 x 8 groups of 8, bf16 (32 bytes of a row a
+    // block): 45.0 / 34.6 us; of 1000 (64 bytes): 19.3 / 23.8.
+    const int most_quads = k.v == 8 ? 1 : k.v == 4 ? 2 : 4;
+    if (lpg <= slab_threads && held(slab_threads, 1) <= most_quads) {
+        // As few groups a block as there are, for more blocks; more where blocks
+        // abound and a row's share is under a 64-byte line or a block under 256
+        // threads.
         int per = 1;
-        while (per * 2 <= groups && per * a.cg * elem < 64 && samples * (groups / (per * 2)) >= 512 &&
-               held(slab_threads, per * 2) <= kSlabQuads)
+        while (per * 2 <= groups && samples * (groups / (per * 2)) >= 256 && held(slab_threads, per * 2) <= 1 &&
+               (per * a.cg * elem < 64 || per * lpg * quads < 256))
             per *= 2;
-        // one wave where it holds the slab in one go, else the size at which a
-        // thread holds one quad
-        k.threads = 64;
-        while (k.threads < slab_threads && held(k.threads, per) > 1) k.threads *= 2;
-        const int64_t q = held(k.threads, per);
-        k.quads = q <= 1 ? 1 : q <= 2 ? 2 : 4;
-        a.lanes = per * lpg;
-        a.ty = k.threads / a.lanes;
-        a.chunks = (groups + per - 1) / per;
-        return k;
+        if (samples * ((groups + per - 1) / per) <= 512 || per * a.cg * elem >= 64 || per == groups) {
+            k.slab = true;
+            // the smallest block at which a thread holds one quad
+            k.threads = 64;
+            while (k.threads < slab_threads && held(k.threads, per) > 1) k.threads *= 2;
+            const int64_t q = held(k.threads, per);
+            k.quads = q <= 1 ? 1 : q <= 2 ? 2 : 4;
+            a.lanes = per * lpg;
+            a.ty = k.threads / a.lanes;
+            a.chunks = (groups + per - 1) / per;
+            return k;
+        }
     }
     if (lpg <= kNormThreads) {
         int per = kNormThreads / lpg;

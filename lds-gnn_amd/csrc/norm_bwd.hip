@@ -397,12 +397,8 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
                         hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
                                            dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
                                            rstd, sums);
-                    else if (k.quads == 1)
-                        slab(IntC<1>{});
-                    else if (k.quads == 2)
-                        slab(IntC<2>{});
                     else
-                        slab(IntC<4>{});
+                        with_quads<V>(k.quads, slab);
                     if (cblocks)
                         hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3((unsigned)cblocks), dim3(kNormThreads), 0, st,
                                            (const float2*)sums, a, pairs, means, dweight, dbias);

@@ -299,12 +299,8 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
                         hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>),
                                            dim3((unsigned)(samples * b.parts * b.chunks)), dim3(kNormThreads), 0, st,
                                            (const T*)x, b, mean, rstd, (T*)y);
-                    else if (k.quads == 1)
-                        slab(IntC<1>{});
-                    else if (k.quads == 2)
-                        slab(IntC<2>{});
                     else
-                        slab(IntC<4>{});
+                        with_quads<V>(k.quads, slab);
                 };
                 drop ? go(BoolC<true>{}) : go(BoolC<false>{});
                 LDS_RETURN_LAST_ERROR();

@@ -556,7 +556,8 @@ def test_int8_matmul_empty(device, ops, m, n, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape,n", [((1, 64), 16), ((37,), 5), ((2, 9, 100), 33), ((300, 1433), 16), ((1, 4096), 260)])
+@pytest.mark.parametrize("shape,n", [((1, 64), 16), ((37,), 5), ((1, 1), 1), ((3, 17), 40), ((4, 8200), 33),
+                                     ((2, 20000), 7), ((4, 5000), 100), ((1, 40000), 19), ((5, 130), 18), ((2, 9, 100), 33), ((300, 1433), 16), ((1, 4096), 260)])
 def test_int8_linear(device, ops, dtype, shape, n):
     """The quantised operands are those of quantize64 exactly; the rest as in
     test_int8_matmul_scales.  Rows of zeros give the bias, rows with a NaN give
