@@ -9,17 +9,17 @@
 namespace lds {
 
 // x - mean and h / scale of a quad.
-template <typename T, int V, int ACT, bool DROP>
+template <typename T, int V, int ACT, bool DROP, bool SPAN>
 struct BackQuad {
     float d[4][V], h[4][V];
 
-    __device__ __forceinline__ void eval(const Quad<T, V>& x, const Quad<T, V>& g, const NormParams<V>& par, float mu,
-                                         const bool (&kept)[4][V]) {
+    __device__ __forceinline__ void eval(const Quad<T, V>& x, const Quad<T, V>& g, const NormParams<V>& par,
+                                         const GroupValue<V, SPAN>& mu, const bool (&kept)[4][V]) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                d[r][e] = elem<T, V>(x.row[r], e) - mu;
+                d[r][e] = elem<T, V>(x.row[r], e) - mu[e];
                 float t = elem<T, V>(g.row[r], e);
                 if constexpr (DROP) t = kept[r][e] ? t : 0.f;
                 if constexpr (ACT == LDS_ACT_RELU) {
@@ -43,15 +43,16 @@ struct BackQuad {
         }
     }
     // dx = (γ rstd scale) h + (-(rstd² m2) (x - mean) - rstd m1)
-    __device__ __forceinline__ void store(const QuadRows& in, const float (&rws)[V], float k0, float k1,
-                                          T* __restrict__ at, int64_t ld) const {
+    __device__ __forceinline__ void store(const QuadRows& in, const float (&rws)[V], const GroupValue<V, SPAN>& k0,
+                                          const GroupValue<V, SPAN>& k1, T* __restrict__ at, int64_t ld,
+                                          int skip) const {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (r < in.lo || r >= in.hi) continue;
             float o[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(rws[e], h[r][e], __builtin_fmaf(k1, d[r][e], k0));
-            store_vec<T, V>(at + r * ld, o);
+            for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(rws[e], h[r][e], __builtin_fmaf(k1[e], d[r][e], k0[e]));
+            store_own<T, V, SPAN>(at + r * ld, skip, o);
         }
     }
 };
@@ -62,12 +63,13 @@ struct QuadPair {
 };
 
 // A thread's channel sums from those of BackQuad::sums.
-template <int V>
-__device__ __forceinline__ void finish_sums(float (&sh)[V], float (&sx)[V], float scale, float rs) {
+template <int V, bool SPAN>
+__device__ __forceinline__ void finish_sums(float (&sh)[V], float (&sx)[V], float scale,
+                                            const GroupValue<V, SPAN>& rs) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         sh[e] *= scale;
-        sx[e] *= scale * rs;
+        sx[e] *= scale * rs[e];
     }
 }
 
@@ -138,17 +140,17 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
             g[k].load(gs, lddy, p, q, in);
         }
     }
-    float mu = 0.f, rs = 0.f;
+    GroupValue<V, false> mu{}, rs{};
     NormParams<V> par{};
     const float scale = DROP ? a.key.scale : 1.f;
     float sh[V] = {}, sx[V] = {};
     if (p.live) {
-        mu = mean[s * a.groups + p.group];
-        rs = rstd[s * a.groups + p.group];
+        mu.f[0] = mean[s * a.groups + p.group];
+        rs.f[0] = rstd[s * a.groups + p.group];
         par.load(a, p.c0);
         par.times(rs);
     }
-    BackQuad<T, V, ACT, DROP> b;
+    BackQuad<T, V, ACT, DROP, false> b;
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
         const int64_t q = p.q0 + p.ty + k * a.ty;
@@ -181,7 +183,8 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
     m = group_sum<float2, NT>(m, a, p, red, blockDim.x);
     const float inv = 1.f / ((float)a.n * (float)a.cg);
     if (!p.live) return;
-    const float k0 = -m.x * inv, k1 = -rs * (m.y * inv);  // of γ rstd: one rstd is in the sums
+    // of γ rstd: one rstd is in the sums
+    const GroupValue<V, false> k0{{-m.x * inv}}, k1{{-rs[0] * (m.y * inv)}};
 #pragma unroll
     for (int e = 0; e < V; ++e) par.rw[e] *= Q > 1 ? 1.f : scale;
     T* ds = dx + p.c0;
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
         float rws[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) rws[e] = Q > 1 ? par.rw[e] * scale : par.rw[e];
-        b.store(quad_rows(p, q), rws, k0, k1, ds + 4 * q * a.c, a.c);
+        b.store(quad_rows(p, q), rws, k0, k1, ds + 4 * q * a.c, a.c, 0);
     }
 }
 
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
 // parts
 // ---------------------------------------------------------------------------
 
-template <typename T, int V, int ACT, bool DROP>
+template <typename T, int V, int ACT, bool DROP, bool SPAN>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __restrict__ dy, int64_t sdy,
                                                                    int64_t lddy, const T* __restrict__ x, NormArgs a,
                                                                    const float* __restrict__ mean,
@@ -215,7 +218,9 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __re
     const NormPlace p = norm_part_place(a, V);
     float sh[V] = {}, sx[V] = {};
     if (p.live) {
-        const float mu = mean[p.s * a.groups + p.group], rs = rstd[p.s * a.groups + p.group];
+        GroupValue<V, SPAN> mu, rs;
+        mu.fill(a, p, [&](int g) { return mean[p.s * a.groups + g]; });
+        rs.fill(a, p, [&](int g) { return rstd[p.s * a.groups + g]; });
         NormParams<V> par;
         par.load(a, p.c0);
         ColumnKeep<V> columns;
@@ -232,16 +237,24 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_sums_kernel(const T* __re
             [&](const QuadPair<T, V>& d, int64_t q, const QuadRows in) {
             bool kept[4][V];
             if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-            BackQuad<T, V, ACT, DROP> b;
+            BackQuad<T, V, ACT, DROP, SPAN> b;
             b.eval(d.x, d.g, par, mu, kept);
             b.sums(in, sh, sx);
         });
         finish_sums<V>(sh, sx, DROP ? a.key.scale : 1.f, rs);
     }
-    const int c0 = chunk_first(a, p.chunk, V), c1 = chunk_last(a, p.chunk);
-    channel_sums<V, kNormThreads>(sh, sx, a, red, kNormThreads, [&](int i, float h, float hx) {
-        if (c0 + i < c1) out[(p.s * a.parts + p.part) * a.c + c0 + i] = make_float2(h, hx);
-    });
+    float2* sums = out + (p.s * a.parts + p.part) * a.c;
+    if constexpr (SPAN) {
+        channel_sums<V, kNormThreads>(sh, sx, a, red, kNormThreads, [&](int i, float h, float hx) {
+            const int at = i - i % V, first = at < a.c - V ? at : a.c - V, c = first + i % V;
+            if (c >= at) sums[c] = make_float2(h, hx);  // a channel's owner
+        });
+    } else {
+        const int c0 = chunk_first(a, p.chunk, V), c1 = chunk_last(a, p.chunk);
+        channel_sums<V, kNormThreads>(sh, sx, a, red, kNormThreads, [&](int i, float h, float hx) {
+            if (c0 + i < c1) sums[c0 + i] = make_float2(h, hx);
+        });
+    }
 }
 
 // Blocks [0, pairs): a (sample, group)'s two means.  The blocks after them: four
@@ -305,7 +318,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
     }
 }
 
-template <typename T, int V, int ACT, bool DROP>
+template <typename T, int V, int ACT, bool DROP, bool SPAN>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __restrict__ dy, int64_t sdy, int64_t lddy,
                                                                  const T* __restrict__ x, NormArgs a,
                                                                  const float* __restrict__ mean,
@@ -314,12 +327,13 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
                                                                  T* __restrict__ dx) {
     const NormPlace p = norm_part_place(a, V);
     if (!p.live) return;
-    const float mu = mean[p.s * a.groups + p.group], rs = rstd[p.s * a.groups + p.group];
+    GroupValue<V, SPAN> mu, rs, k0, k1;
+    mu.fill(a, p, [&](int g) { return mean[p.s * a.groups + g]; });
+    rs.fill(a, p, [&](int g) { return rstd[p.s * a.groups + g]; });
     NormParams<V> par;
     par.load(a, p.c0);
     ColumnKeep<V> columns;
     if constexpr (DROP) columns.init(a.key, (uint32_t)p.c0);
-    const float2 m = means[p.s * a.groups + p.group];
     const T* xs = x + p.s * a.sx + p.c0;
     const T* gs = dy + p.s * sdy + p.c0;
     T* ds = dx + p.c0;
@@ -327,7 +341,11 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
     float rws[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) rws[e] = DROP ? par.rw[e] * a.key.scale : par.rw[e];
-    const float k0 = -rs * m.x, k1 = -rs * rs * m.y;
+    k0.fill(a, p, [&](int g) { return -rstd[p.s * a.groups + g] * means[p.s * a.groups + g].x; });
+    k1.fill(a, p, [&](int g) {
+        const float r = rstd[p.s * a.groups + g];
+        return -r * r * means[p.s * a.groups + g].y;
+    });
     each_quad_ahead<QuadPair<T, V>>(
         a, p,
         [&](QuadPair<T, V>& d, int64_t q, const QuadRows in) {
@@ -337,9 +355,9 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
         [&](const QuadPair<T, V>& d, int64_t q, const QuadRows in) {
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-        BackQuad<T, V, ACT, DROP> b;
+        BackQuad<T, V, ACT, DROP, SPAN> b;
         b.eval(d.x, d.g, par, mu, kept);
-        b.store(in, rws, k0, k1, ds + 4 * q * a.c, a.c);
+        b.store(in, rws, k0, k1, ds + 4 * q * a.c, a.c, p.skip);
     });
 }
 
@@ -380,8 +398,9 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
     float2* means = k.slab ? nullptr : sums + samples * a.parts * (int64_t)c;
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
-        return with_vec<16 / (int)sizeof(T)>(k.v, [&](auto vc) -> int {
+        return with_vec<16 / (int)sizeof(T)>(k.v, a.span, [&](auto vc, auto sc) -> int {
             constexpr int V = decltype(vc)::value;
+            constexpr bool SPAN = decltype(sc)::value;
             return with_act(act, [&](auto ac) -> int {
                 constexpr int ACT = decltype(ac)::value;
                 auto go = [&](auto dr) {
@@ -394,16 +413,16 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
                                            direct ? dweight : nullptr, direct ? dbias : nullptr, (T*)dx);
                     };
                     if (!k.slab)
-                        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
+                        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP, SPAN>), dim3((unsigned)blocks),
                                            dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
                                            rstd, sums);
-                    else
+                    else if constexpr (!SPAN)
                         with_quads<V>(k.quads, slab);
                     if (cblocks)
                         hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3((unsigned)cblocks), dim3(kNormThreads), 0, st,
                                            (const float2*)sums, a, pairs, means, dweight, dbias);
                     if (!k.slab && dx)
-                        hipLaunchKernelGGL((gn_bwd_dx_kernel<T, V, ACT, DROP>), dim3((unsigned)blocks),
+                        hipLaunchKernelGGL((gn_bwd_dx_kernel<T, V, ACT, DROP, SPAN>), dim3((unsigned)blocks),
                                            dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
                                            rstd, (const float2*)means, (T*)dx);
                 };

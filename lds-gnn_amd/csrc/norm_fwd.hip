@@ -10,21 +10,21 @@ struct Moments {
 };
 
 // y of a quad from x.
-template <typename T, int V, int ACT, bool DROP>
-__device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& in, const NormParams<V>& par, float mu,
-                                           const bool (&kept)[4][V], float scale, T* __restrict__ at,
-                                           int64_t ld) {
+template <typename T, int V, int ACT, bool DROP, bool SPAN>
+__device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& in, const NormParams<V>& par,
+                                           const GroupValue<V, SPAN>& mu, const bool (&kept)[4][V], float scale,
+                                           T* __restrict__ at, int64_t ld, int skip) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if (r < in.lo || r >= in.hi) continue;
         float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float z = __builtin_fmaf(elem<T, V>(x.row[r], e) - mu, par.rw[e], par.b[e]);
+            const float z = __builtin_fmaf(elem<T, V>(x.row[r], e) - mu[e], par.rw[e], par.b[e]);
             o[e] = act_f<ACT>(z);
             if constexpr (DROP) o[e] = kept[r][e] ? o[e] * scale : 0.f;
         }
-        store_vec<T, V>(at + r * ld, o);
+        store_own<T, V, SPAN>(at + r * ld, skip, o);
     }
 }
 
@@ -92,7 +92,8 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, 
     const float off = d2.x * inv, mu = m0 + off;
     const float rs = 1.f / sqrtf(fmaxf(__builtin_fmaf(-off, off, d2.y * inv), 0.f) + eps);
     if (!p.live) return;
-    par.times(rs);
+    GroupValue<V, false> gmu{{mu}};
+    par.times(GroupValue<V, false>{{rs}});
     if (p.ty == 0 && p.c0 == p.group * a.cg) {
         mean[s * a.groups + p.group] = mu;
         rstd[s * a.groups + p.group] = rs;
@@ -104,7 +105,8 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, 
         if (q >= p.q1) continue;
         bool kept[4][V];
         if constexpr (DROP) unpack_kept<V>(masks[k], kept);
-        apply_quad<T, V, ACT, DROP>(v[k], quad_rows(p, q), par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c);
+        apply_quad<T, V, ACT, DROP, false>(v[k], quad_rows(p, q), par, gmu, kept, a.key.scale, ys + 4 * q * a.c, a.c,
+                                           0);
     }
 }
 
@@ -182,6 +184,93 @@ __global__ __launch_bounds__(kNormThreads) void gn_stats_kernel(const T* __restr
             Moments{gm, (float)c, (float)g2};
 }
 
+// The same where vectors lie across groups: running moments per channel, about
+// the channel's first value, put together per group at the end.
+template <typename T, int V>
+__global__ __launch_bounds__(kNormThreads) void gn_stats_span_kernel(const T* __restrict__ x, NormArgs a,
+                                                                     Moments* __restrict__ out) {
+    __shared__ double s_mean[V][kNormThreads];
+    __shared__ float s_m2[V][kNormThreads], s_cnt[kNormThreads];
+    const NormPlace p = norm_part_place(a, V);
+    float k[V], mean[V] = {}, m2[V] = {}, cnt = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) k[e] = 0.f;
+    if (p.live) {
+        const T* xs = x + p.s * a.sx + p.c0;
+        each_quad(a, p, [&](int64_t q, const QuadRows in) {
+            Quad<T, V> v;
+            v.load(xs, a.ldx, p, q, in);
+            if (cnt == 0.f) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) k[e] = elem<T, V>(v.row[0], e);
+            }
+            const float m = (float)(in.hi - in.lo), over = __builtin_amdgcn_rcpf(m);
+            const float part = m * __builtin_amdgcn_rcpf(cnt + m), both = cnt * part;
+            float use[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) use[r] = r >= in.lo && r < in.hi ? 1.f : 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float d[4], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    d[r] = elem<T, V>(v.row[r], e) - k[e];
+                    s1 = __builtin_fmaf(use[r], d[r], s1);
+                }
+                const float mq = s1 * over;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float t = use[r] * (d[r] - mq);
+                    s2 = __builtin_fmaf(t, t, s2);
+                }
+                const float delta = mq - mean[e];
+                mean[e] = __builtin_fmaf(delta, part, mean[e]);
+                m2[e] += __builtin_fmaf(delta * delta, both, s2);
+            }
+            cnt += m;
+        });
+    }
+    s_cnt[threadIdx.x] = cnt;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        s_mean[e][threadIdx.x] = (double)k[e] + (double)mean[e];
+        s_m2[e][threadIdx.x] = m2[e];
+    }
+    __syncthreads();
+    // a team of lanes per group over its channels in the ty rows of threads
+    const int members = a.ty * a.cg;
+    int team = kWave;
+    while (team > 1 && (team / 2 >= members || a.groups * team > 2 * kNormThreads)) team /= 2;
+    const int lane = threadIdx.x & (team - 1);
+    const int end = (a.lanes - 1) * V;  // the last vector ends with the row
+    for (int g = threadIdx.x / team; g < a.groups; g += kNormThreads / team) {
+        const auto each = [&](auto&& f) {
+            for (int i = lane; i < members; i += team) {
+                const int r = (int)((unsigned)i / (unsigned)a.cg), c = g * a.cg + (i - r * a.cg);
+                const int vec = c < end ? c / V : a.lanes - 1, e = c < end ? c % V : c - (a.c - V);
+                const int t = r * a.lanes + vec;
+                if (s_cnt[t] > 0.f) f(s_cnt[t], s_mean[e][t], s_m2[e][t]);
+            }
+        };
+        double n = 0.0, mu = 0.0, v = 0.0;
+        each([&](float c, double m, float) {
+            n += (double)c;
+            mu += (double)c * m;
+        });
+        for (int o = team / 2; o > 0; o >>= 1) {
+            n += __shfl_xor(n, o);
+            mu += __shfl_xor(mu, o);
+        }
+        mu /= n > 0.0 ? n : 1.0;
+        each([&](float c, double m, float q) {
+            const double d = m - mu;
+            v += (double)q + (double)c * d * d;
+        });
+        for (int o = team / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+        if (lane == 0) out[(p.s * a.groups + g) * (int64_t)a.parts + p.part] = Moments{mu, (float)n, (float)v};
+    }
+}
+
 // One wave per (sample, group): its parts combined in fp64.
 __global__ __launch_bounds__(kNormThreads) void gn_combine_kernel(const Moments* __restrict__ in, int64_t total,
                                                                   int parts, float eps, float* __restrict__ mean,
@@ -211,14 +300,15 @@ __global__ __launch_bounds__(kNormThreads) void gn_combine_kernel(const Moments*
     }
 }
 
-template <typename T, int V, int ACT, bool DROP>
+template <typename T, int V, int ACT, bool DROP, bool SPAN>
 __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restrict__ x, NormArgs a,
                                                                 const float* __restrict__ mean,
                                                                 const float* __restrict__ rstd, T* __restrict__ y) {
     const NormPlace p = norm_part_place(a, V);
     if (!p.live) return;
-    const float mu = mean[p.s * a.groups + p.group];
-    const float rs = rstd[p.s * a.groups + p.group];
+    GroupValue<V, SPAN> mu, rs;
+    mu.fill(a, p, [&](int g) { return mean[p.s * a.groups + g]; });
+    rs.fill(a, p, [&](int g) { return rstd[p.s * a.groups + g]; });
     NormParams<V> par;
     par.load(a, p.c0);
     ColumnKeep<V> columns;
@@ -231,7 +321,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restr
         v.load(xs, a.ldx, p, q, in);
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-        apply_quad<T, V, ACT, DROP>(v, in, par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c);
+        apply_quad<T, V, ACT, DROP, SPAN>(v, in, par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c, p.skip);
     });
 }
 
@@ -278,11 +368,16 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     LDS_CHECK_ARG(pairs < (int64_t)1 << 32);
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
-        return with_vec<16 / (int)sizeof(T)>(k.v, [&](auto vc) -> int {
+        return with_vec<16 / (int)sizeof(T)>(k.v, a.span, [&](auto vc, auto sc) -> int {
             constexpr int V = decltype(vc)::value;
+            constexpr bool SPAN = decltype(sc)::value;
             if (!k.slab) {
-                hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0, st,
-                                   (const T*)x, a, (Moments*)ws);
+                if constexpr (SPAN)
+                    hipLaunchKernelGGL((gn_stats_span_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0,
+                                       st, (const T*)x, a, (Moments*)ws);
+                else
+                    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0, st,
+                                       (const T*)x, a, (Moments*)ws);
                 hipLaunchKernelGGL(gn_combine_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(kNormThreads), 0, st,
                                    (const Moments*)ws, pairs, a.parts * a.sub, eps, mean, rstd);
             }
@@ -296,10 +391,10 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
                                            mean, rstd);
                     };
                     if (!k.slab)
-                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP>),
+                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP, SPAN>),
                                            dim3((unsigned)(samples * b.parts * b.chunks)), dim3(kNormThreads), 0, st,
                                            (const T*)x, b, mean, rstd, (T*)y);
-                    else
+                    else if constexpr (!SPAN)
                         with_quads<V>(k.quads, slab);
                 };
                 drop ? go(BoolC<true>{}) : go(BoolC<false>{});

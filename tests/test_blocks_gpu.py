@@ -167,6 +167,7 @@ NORM_SHAPES = [  # samples, n, groups, channels per group
     (1, 1, 1, 1), (1, 1, 32, 8), (3, 1, 2, 3), (2, 7, 4, 5), (1, 5, 1, 2), (5, 33, 3, 16), (2, 100, 1, 700),
     (1, 9, 2, 4096), (1, 3, 1, 2051), (4, 515, 12, 5), (1, 2708, 4, 4), (2, 600, 32, 8), (17, 2, 300, 2),
     (9, 1501, 3, 7), (1, 9001, 2, 4), (2, 5003, 2, 16), (1, 40, 1, 8200),
+    (2, 6001, 3, 7), (1, 7011, 12, 5), (3, 5001, 5, 3), (1, 4502, 4, 12), (1, 18000, 1, 9), (2, 1500, 1, 33),
 ]
 
 
@@ -331,10 +332,11 @@ def test_group_norm_samples_stand_alone(device, ops):
     assert torch.allclose(y[2, :, 24:], (b * torch.sigmoid(b))[24:].expand(40, 8), rtol=1e-6, atol=1e-7)
 
 
-def test_group_norm_far_from_zero(device, ops):
+@pytest.mark.parametrize("n,cg", [(700, 8), (9000, 8), (9000, 5)])
+def test_group_norm_far_from_zero(device, ops, n, cg):
     """Mean 3000 sd, one outlier among the first values: the bound of
     norm_bounds, whose term in |mean| is the mean's own last bit."""
-    x, w, b, _ = norm_inputs(2, 700, 2, 8, torch.float32, seed=8, offset=0.0)
+    x, w, b, _ = norm_inputs(2, n, 2, cg, torch.float32, seed=8, offset=0.0)
     x = x / 1.5 + 3000.0
     x[:, 0, 0] = 9000.0
     y = ops.group_norm_act(x.to(device), 2, w.to(device), b.to(device)).cpu()
