@@ -11,10 +11,9 @@ namespace lds {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
-// q = x / s to the nearest integer, ties to even, of the exact quotient.  t = x · (1/s)
-// is within 127 · 2^-22 of it, so only a t that close to a half is looked at again:
-// there the sign of x - (q ± ½) s, one fused operation, decides.
-__device__ __forceinline__ float quant_one(float x, float s, float inv) {
+// q = x / s to the nearest integer, ties to even, of the exact quotient: the
+// sign of x - (q ± ½) s, one fused operation, decides next to a half.
+__device__ __forceinline__ int quant_exact(float x, float s, float inv) {
     const float t = x * inv;
     float q = rintf(t);
     const float d = t - q;
@@ -23,7 +22,7 @@ __device__ __forceinline__ float quant_one(float x, float s, float inv) {
         const float r = __builtin_fmaf(-h, s, x);
         q = r > 0.f ? h + 0.5f : r < 0.f ? h - 0.5f : rintf(h);
     }
-    return fminf(fmaxf(q, -127.f), 127.f);
+    return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
 
 // A row's scale from the bits of its largest |x|, and what quantises its values.
@@ -41,13 +40,44 @@ struct RowScale {
         su = s * up;
         inv = zero ? 0.f : 1.f / su;
     }
+    // V values as bytes.  Adding 1.5 2^23 rounds x (1/s) to an integer (ties to
+    // even) that then stands in the low bits.  x (1/s) is within 127 2^-22 of the
+    // quotient, so only a vector with a value that close to a half (one in a
+    // few thousand), or of a row with a tiny scale, is done again exactly.
+    // |q| <= 127 needs no clamp: the largest quotient is 127 to within 2^-16.
     template <int V>
     __device__ __forceinline__ void put(signed char* __restrict__ q, const float (&f)[V]) const {
-        typedef signed char cv __attribute__((ext_vector_type(V)));
-        cv o;
+        constexpr float kRound = 12582912.f;
+        static_assert(V % 4 == 0, "whole words");
+        uint32_t o[V / 4];
+        float off = up != 1.f ? 1.f : 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = zero ? (signed char)0 : (signed char)(int)quant_one(f[e] * up, su, inv);
-        *reinterpret_cast<cv*>(q) = o;
+        for (int w = 0; w < V / 4; ++w) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float r = __builtin_fmaf(f[4 * w + e], inv, kRound);
+                off = fmaxf(off, fabsf(__builtin_fmaf(f[4 * w + e], inv, -(r - kRound))));
+                y[e] = __float_as_uint(r);
+            }
+            const uint32_t lo = __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(y[3], y[2], 0x04000c0cu);
+            o[w] = lo | hi;
+        }
+        if (off > 0.4999f) {
+#pragma unroll
+            for (int w = 0; w < V / 4; ++w) {
+                o[w] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    o[w] |= ((uint32_t)quant_exact(f[4 * w + e] * up, su, inv) & 0xffu) << (8 * e);
+            }
+        }
+        typedef uint32_t words __attribute__((ext_vector_type(V / 4)));
+        words v;
+#pragma unroll
+        for (int w = 0; w < V / 4; ++w) v[w] = zero ? 0u : o[w];
+        *reinterpret_cast<words*>(q) = v;
     }
 };
 template <int V>
