@@ -90,6 +90,26 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top, const float (&f)[V]) 
     return top;
 }
 
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// The largest of G neighbouring lanes (16, 32 or 64), in each of them: within
+// rows of 16 lanes by DPP, across them by the lane swaps; no LDS round trips.
+template <int G>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    v = umax(v, (uint32_t)dpp_int<0x128>((int)v));  // row_ror:8, 4, 2, 1
+    v = umax(v, (uint32_t)dpp_int<0x124>((int)v));
+    v = umax(v, (uint32_t)dpp_int<0x122>((int)v));
+    v = umax(v, (uint32_t)dpp_int<0x121>((int)v));
+    if constexpr (G >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = umax(r[0], r[1]);
+    }
+    if constexpr (G >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = umax(r[0], r[1]);
+    }
+    return v;
+}
+
 // G lanes per row (a power of two up to the block), R vectors of V values a lane
 // held in registers between the two uses of a row; a row longer than G R V is
 // read again.  The largest |x| is found on the bits, so that an infinity or a
@@ -122,16 +142,12 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
         load_part<T, V>(xr + j, cols - (int)j, f);
         top = top_bits<V>(top, f);
     }
-#pragma unroll
-    for (int o = (G < 64 ? G : 64) / 2; o > 0; o >>= 1) {
-        const uint32_t b = __shfl_xor(top, o);
-        top = b > top ? b : top;
-    }
+    top = lanes_max<(G < 64 ? G : 64)>(top);
     if constexpr (G > 64) {
         if (wave_lane() == 0) red[wave_id()] = top;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = red[i] > top ? red[i] : top;
+        for (int i = 0; i < 4; ++i) top = umax(top, red[i]);
     }
     if (!live) return;
     const RowScale k(top);
@@ -312,11 +328,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(const TX* __restrict__ x,
                 load_part<TX, V>(x + i * ldx + j, a.k - j, g);
                 top[i] = top_bits<V>(top[i], g);
             }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint32_t b = __shfl_xor(top[i], o);
-            top[i] = b > top[i] ? b : top[i];
-        }
+        top[i] = lanes_max<64>(top[i]);
         if (lane == 0) tops[w][i] = top[i];
     }
     __syncthreads();
@@ -325,7 +337,7 @@ __global__ __launch_bounds__(512) void int8_few_kernel(const TX* __restrict__ x,
         if (i >= m) break;
         uint32_t b = 0;
 #pragma unroll
-        for (int u = 0; u < W; ++u) b = tops[u][i] > b ? tops[u][i] : b;
+        for (int u = 0; u < W; ++u) b = umax(b, tops[u][i]);
         const RowScale k(b);
         if (t == 0) scales[i] = k.s;
         signed char* qr = xq + i * ldq;
@@ -518,10 +530,6 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* 
     // neighbouring ones.  Unit u of row r (16 bytes) sits at place u ^ (r % 16).
     static_assert(FN == 2 && kStages * kStageBytes >= kWaves * 8192, "an 8 KB region per wave");
     constexpr int VO = 16 / (int)sizeof(T), kRowLanes = 64 / VO, kRows = 64 / kRowLanes;
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);
-    __builtin_amdgcn_s_barrier();  // every wave has read its last operands
-    asm volatile("" ::: "memory");
     signed char* region = smem + w * 8192;
     const int oc = lane % kRowLanes, orow = lane / kRowLanes;
     const int col = n0 + wn * 64 + oc * VO;
@@ -536,6 +544,17 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* 
 #pragma unroll
         for (int e = 0; e < VO; ++e) b[e] = load_param(a.bias, a.ptype, col + e < a.n ? col + e : a.n - 1);
     }
+    // the row scales of all the lane's rows at once: one wait, not one a row
+    float xs[FM * 32 / kRows];
+#pragma unroll
+    for (int i = 0; i < FM * 32 / kRows; ++i) {
+        const int64_t row = m0 + wm * (BM / WM) + i * kRows + orow;
+        xs[i] = a.xs[row < a.m ? row : a.m - 1];
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    __builtin_amdgcn_s_barrier();  // every wave has read its last operands
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -553,14 +572,13 @@ __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* 
             const int r = q * kRows + orow;
             const int64_t row = m0 + wm * (BM / WM) + 32 * i + r;
             if (row < a.m && col < a.n) {
-                const float xs = a.xs[row];
                 float o[VO];
 #pragma unroll
                 for (int h = 0; h < VO / 4; ++h) {
                     const v4i v = *reinterpret_cast<const v4i*>(region + r * 256 +
                                                                 ((oc * (VO / 4) + h) ^ (r & 15)) * 16);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * h + e] = (float)v[e] * xs * s[4 * h + e] + b[4 * h + e];
+                    for (int e = 0; e < 4; ++e) o[4 * h + e] = (float)v[e] * xs[i * (32 / kRows) + q] * s[4 * h + e] + b[4 * h + e];
                 }
                 store_part<T, VO>(y + row * a.ldy + col, a.n - col, o);
             }
@@ -609,9 +627,11 @@ extern "C" int lds_quantize_rows(const void* x, int64_t ldx, int64_t rows, int c
             hipLaunchKernelGGL((quantize_rows_kernel<T, V, G, R>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))),
                                dim3(256), 0, (hipStream_t)stream, (const T*)x, ldx, rows, cols, q, ldq, scale);
         };
-        // a row in the registers of 16 lanes, of a wave or of a block
+        // a row in the registers of 16 or 32 lanes, of a wave or of a block
         if (ldq <= 16 * V)
             go(IntC<16>{}, IntC<1>{});
+        else if (ldq <= 32 * V)
+            go(IntC<32>{}, IntC<1>{});
         else if (ldq <= 64 * V)
             go(IntC<64>{}, IntC<1>{});
         else if (ldq <= 64 * V * 4)

@@ -704,7 +704,7 @@ def _int8_stride(k: int) -> int:
     that the 16 rows a wave reads at once do not fall on the same cache sets
     (16 x 4096 x 4096: 5.9 us at stride 4096, 4.8 at 4160); short rows are only
     padded to 16 bytes."""
-    return -(-k // 16) * 16 if k <= 64 else (-(-k // 64) | 1) * 64
+    return -(-k // 16) * 16 if k <= 512 else (-(-k // 64) | 1) * 64
 
 
 def _int8_readable(q: torch.Tensor, what: str) -> torch.Tensor:
