@@ -10,29 +10,6 @@
 
 namespace lds {
 
-// One thread per (column j, row quad): one Philox call covers four rows.
-__global__ __launch_bounds__(256) void dropout_kernel(const float* __restrict__ x, int ldx,
-                                                       float* __restrict__ y, int ldy, int rows,
-                                                       int cols, float keep_prob, float scale,
-                                                       uint32_t k0, uint32_t k1, uint32_t tag,
-                                                       uint32_t counter, int quads) {
-    const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t total = (int64_t)quads * cols;
-    if (t >= total) return;
-    const int rq = (int)(t / cols);
-    const int j = (int)(t - (int64_t)rq * cols);
-    float u[4];
-    philox_quad(k0, k1, tag, counter, (uint32_t)j, (uint32_t)rq, u);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int i = rq * 4 + r;
-        if (i < rows) {
-            const float xv = x[(int64_t)i * ldx + j];
-            y[(int64_t)i * ldy + j] = u[r] < keep_prob ? xv * scale : 0.0f;
-        }
-    }
-}
-
 // y = residual + mask(x), one thread per row quad and 16 bytes of a row: the
 // quad shares its Philox calls, the four rows' loads are independent.
 template <typename T, int V, bool RES, bool DROP>
@@ -70,8 +47,8 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ 
         if (i0 + r >= rows) break;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            float o = v[r][e];
-            if constexpr (DROP) o = kept[r][e] ? o * key.scale : 0.f;
+            float o = v[r][e] * key.scale;
+            if constexpr (DROP) o = kept[r][e] ? o : 0.f;
             if constexpr (RES) o = o + a[r][e];
             v[r][e] = o;
         }
@@ -88,22 +65,6 @@ extern "C" int lds_abi_version(void) { return LDS_ABI_VERSION; }
 extern "C" const char* lds_error_string(int err) {
     const char* s = hipGetErrorString((hipError_t)err);
     return s ? s : "unknown hip error";
-}
-
-extern "C" int lds_dropout(const float* x, int ldx, float* y, int ldy, int rows, int cols,
-                           float keep_prob, float scale, uint64_t seed, uint32_t tag,
-                           uint32_t counter, void* stream) {
-    LDS_CHECK_ARG(x != nullptr && y != nullptr && rows >= 0 && cols >= 0);
-    LDS_CHECK_ARG(ldx >= cols && ldy >= cols);
-    if (rows == 0 || cols == 0) return 0;
-    const int quads = (rows + 3) / 4;
-    const int64_t total = (int64_t)quads * cols;
-    const int64_t blocks = (total + 255) / 256;
-    LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
-    hipLaunchKernelGGL(dropout_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                       x, ldx, y, ldy, rows, cols, keep_prob, scale, (uint32_t)seed,
-                       (uint32_t)(seed >> 32), tag, counter, quads);
-    LDS_RETURN_LAST_ERROR();
 }
 
 extern "C" int lds_dropout_add(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy,
@@ -135,4 +96,15 @@ extern "C" int lds_dropout_add(const void* x, int64_t ldx, const void* residual,
         }
         LDS_RETURN_LAST_ERROR();
     });
+}
+
+extern "C" int lds_dropout(const float* x, int ldx, float* y, int ldy, int rows, int cols,
+                           float keep_prob, float scale, uint64_t seed, uint32_t tag,
+                           uint32_t counter, void* stream) {
+    LDS_CHECK_ARG(x != nullptr && y != nullptr && rows >= 0 && cols >= 0);
+    LDS_CHECK_ARG(ldx >= cols && ldy >= cols);
+    // u lies in [0, 1): a keep_prob past either end keeps all or none
+    keep_prob = keep_prob >= 1.f ? 1.f : keep_prob > 0.f ? keep_prob : 0.f;
+    return lds_dropout_add(x, ldx, nullptr, 0, y, ldy, rows, cols, LDS_F32, keep_prob, scale, seed, tag, counter,
+                           stream);
 }

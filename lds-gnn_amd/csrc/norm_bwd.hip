@@ -272,7 +272,7 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
         const int64_t items = (int64_t)a.parts * a.cg;
 #pragma unroll 4
         for (int64_t i = t; i < items; i += kNormThreads) {
-            const int64_t part = (uint32_t)i / (uint32_t)a.cg;
+            const int64_t part = items <= 0xffffffffll ? (uint32_t)i / (uint32_t)a.cg : i / a.cg;
             const int c = g * a.cg + (int)(i - part * a.cg);
             const float2 v = sums[(s * a.parts + part) * a.c + c];
             const float w = a.weight ? load_param(a.weight, a.ptype, c) : 1.f;

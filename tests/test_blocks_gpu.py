@@ -125,6 +125,62 @@ def test_dropout_gradients(device, ops, dtype):
     assert torch.equal(g2.cpu(), plain_dropout(dy, KEY, 0.25))
 
 
+def test_dropout_entries_at_the_ends(device):
+    """lds_dropout and lds_dropout_add take the scale at its word: keep 1 scales
+    every element, keep 0 leaves none; lds_dropout takes any keep."""
+    from ldsgnn import _native as nat
+    x = torch.randn(9, 21, device=device)
+    y = torch.empty_like(x)
+    st = nat.stream_of(x.device)
+    for keep, ref in ((1.0, x * 3), (0.0, x * 0), (1.5, x * 3), (-0.5, x * 0)):
+        nat.call("lds_dropout", x.data_ptr(), 21, y.data_ptr(), 21, 9, 21, keep, 3.0, 1, 2, 3, st)
+        assert torch.equal(y, ref), keep
+        if 0.0 <= keep <= 1.0:
+            nat.call("lds_dropout_add", x.data_ptr(), 21, 0, 0, y.data_ptr(), 21, 9, 21, 0, keep, 3.0, 1, 2, 3, st)
+            assert torch.equal(y, ref), keep
+
+
+def test_offsets_past_32_bits(device, ops):
+    """More than 2^31 elements: the last rows are the definition's."""
+    rows, cols = 70001, 32768
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=device)
+    x.copy_(torch.arange(cols, device=device).remainder(251).to(torch.bfloat16)[None, :])
+    y = ops.keyed_dropout(x, 0.5, KEY, residual=x)
+    tail = 5  # rows 69996 ..: the mask of the last two row quads
+    c = np.arange(cols)
+    ref = torch.empty(tail, cols)
+    for i in range(tail):
+        r = rows - tail + i
+        w = philox.philox4x32_10(c, r >> 2, KEY[1], KEY[2], KEY[0] & 0xFFFFFFFF, KEY[0] >> 32)[r & 3]
+        kept = torch.from_numpy((w >> np.uint64(8)).astype(np.float64) * 2.0 ** -24 < 0.5)
+        xr = x[r].cpu().float()
+        ref[i] = torch.where(kept, xr * 2, torch.zeros_like(xr)) + xr
+    assert torch.equal(y[-tail:].cpu(), ref.to(torch.bfloat16))
+    del y
+    # group norm: the last group of the last sample; its gradient of ones through a constant is 0
+    x3 = x[:70000].view(2, 35000, cols)
+    x3[1, :, -64:] = torch.randn(35000, 64, device=device).to(torch.bfloat16)
+    z = ops.group_norm_act(x3, cols // 64, act="silu")
+    v = x3[1, :, -64:].double()
+    zr = (v - v.mean()) / (v.var(unbiased=False) + 1e-5).sqrt()
+    ref = zr * torch.sigmoid(zr)
+    assert ((z[1, :, -64:].double() - ref).abs() <= HALF[torch.bfloat16] * ref.abs() + 1e-5).all()
+    stats = ops._norm_forward(x3, None, None, ops._NormPlan(cols // 64, 2, 1e-5, 1.0, 1.0, None))[1]
+    del z
+    dy = torch.ones_like(x3)
+    dx, _, _ = ops._norm_backward(dy, x3, None, None, stats, ops._NormPlan(cols // 64, 0, 1e-5, 1.0, 1.0, None),
+                                  (True, False, False))
+    # h = 1: dx = r (1 - 1 - x̂ mean(x̂)), which is 0 to the roundings of the two means
+    assert float(dx[1, :, -64:].abs().max()) <= 1e-4
+    del dx, dy, x3, x
+    a = torch.randint(-127, 128, (rows, 64), dtype=torch.int8, device=device)
+    b = torch.randint(-127, 128, (cols, 64), dtype=torch.int8, device=device)
+    one = torch.ones(rows, device=device)
+    p = ops.int8_matmul(a, one, b, one[:cols], out_dtype=torch.bfloat16)
+    ref = a[-300:].double() @ b.double().t()
+    assert torch.equal(p[-300:], ref.float().to(torch.bfloat16))
+
+
 # ---------------------------------------------------------------------------
 # group norm + activation
 # ---------------------------------------------------------------------------
