@@ -110,6 +110,8 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     return v;
 }
 
+// Bound by memory where rows are long (20000 x 4096 bf16: 42.5 us, 5.8 TB/s), by the
+// waves' latency where they are short (20000 x 128: 4.3 us).
 // G lanes per row (a power of two up to the block), R vectors of V values a lane
 // held in registers between the two uses of a row; a row longer than G R V is
 // read again.  The largest |x| is found on the bits, so that an infinity or a
@@ -204,7 +206,8 @@ __device__ __forceinline__ void put_y(const Int8Args& a, T* __restrict__ y, int6
 }
 
 // A 16 MF x 16 NF tile of y per block; its W waves take W slices of k, four steps of
-// 64 bytes in flight, and meet in LDS.
+// 64 bytes in flight, and meet in LDS.  For few rows, where the weights' bytes
+// are the bound: 1 x 4096 x 4096 4.2 us (4.0 TB/s), 64 rows 7.9 us.
 template <typename T, int MF, int NF, int W>
 __global__ __launch_bounds__(64 * W) void int8_split_kernel(Int8Args a, T* __restrict__ y) {
     constexpr int kAhead = 4;
@@ -392,7 +395,12 @@ __device__ const v4i kZeroChunk = {0, 0, 0, 0};
 //
 // A stage holds the tile's rows of 64 bytes as four 16-byte chunks; chunk c of
 // row r sits at place c ^ (r / 4 % 4), so that the 16 lanes of a read phase, one
-// chunk of 16 rows, meet 16 different 16-byte bank groups.
+// chunk of 16 rows, meet 16 different 16-byte bank groups (no conflict counted).
+//
+// 8192^3: 500 us, 2200 TOP/s (the library's int8 product of that size on the same
+// card: 544 us); 20000 x 4096 x 4096: 340 us, 1970 TOP/s.  Bound by power: with zeros
+// in x and w the latter takes 250 us, at random values the clock is 1.8 GHz and
+// the matrix units are busy 54 % of its cycles.
 template <typename T, int BM, int BN, int WM, int WN, int kStages>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* __restrict__ y) {
     constexpr int kWaves = WM * WN;
