@@ -290,8 +290,8 @@ __global__ __launch_bounds__(64 * W) void int8_split_kernel(Int8Args a, T* __res
 // One or two rows (single nodes): every block quantises the rows into LDS by
 // itself, under the loads of its first weights, and multiplies them with 16
 // rows of w, k split over its eight waves.  One launch: 1 x 4096 x 4096 from
-// bf16 6.7 us, against 8.2 for quantiser and product; two rows 8.1 / 8.4; four
-// rows would be 10.9 / 8.5.
+// bf16 5.4 us, against 7.7 for quantiser and product.  With a slower rounding
+// two rows took 8.1 / 8.4 us and four 10.9 / 8.5, so it ends at two.
 constexpr int kFewRows = 2, kFewBytes = 32768;
 template <typename TX, int V>
 __global__ __launch_bounds__(512) void int8_few_kernel(const TX* __restrict__ x, int64_t ldx, Int8Args a, int ldq,

@@ -2,8 +2,9 @@
 // (norm_fwd.hip) and the backward (norm_bwd.hip) share.
 //
 // A thread owns V neighbouring channels, of one group (V divides the channels
-// per group) or, in the parts form, across groups, and walks row quads: four rows whose flat indices s·n + i differ in
-// their two low bits, the unit in which the keyed dropout mask is drawn.
+// per group) or, in the parts form, across groups, and walks row quads: four
+// rows whose flat indices s·n + i differ in their two low bits, the unit in
+// which the keyed dropout mask is drawn.
 //
 // Two forms.  "Slab": a block keeps a sample's rows of a few groups in its
 // registers, so that x is read once and one launch does it all.  "Parts": a
@@ -33,7 +34,7 @@ struct NormArgs {
     int ty;           // row quads that it takes at a time
     int chunks;       // blocks across a row
     int lpg, sub;     // vectors per group (in the chunk); chunks per group
-    int span;         // vectors lie across groups: see NormPlan
+    int span;         // vectors lie across groups (norm_plan says when)
     int parts;        // row parts per sample
     int64_t part_q;   // row quads per part
     const void* weight;

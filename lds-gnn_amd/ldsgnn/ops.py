@@ -718,7 +718,8 @@ def _int8_readable(q: torch.Tensor, what: str) -> torch.Tensor:
         return q
     ld = q.stride(0) if m > 1 else 16
     if (q.stride(1) == 1 or k == 1) and (ld >= k or m == 1) and ld % 16 == 0 and q.data_ptr() % 16 == 0 and \
-            q.untyped_storage().nbytes() - q.storage_offset() >= (m - 1) * ld + -(-k // 16) * 16:
+            (k % 16 == 0 or
+             q.untyped_storage().nbytes() - q.storage_offset() >= (m - 1) * ld + -(-k // 16) * 16):
         return q
     return _int8_layout(q)
 
