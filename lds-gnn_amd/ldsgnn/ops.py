@@ -424,14 +424,14 @@ def _rows_of(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     a copy only where its strides are no such block's."""
     if t.dim() == 0:
         raise ValueError(f"ldsgnn {what}: expected at least one dimension")
-    cols = t.size(-1)
+    cols, n = t.size(-1), t.numel()
     if cols:
-        rows = t.numel() // cols
+        rows = n // cols
     else:
         rows = 1
         for d in t.shape[:-1]:
             rows *= d
-    if t.is_contiguous() or t.numel() == 0:
+    if n == 0 or t.is_contiguous():
         return t, rows, cols, cols
     try:
         v = t.view(rows, cols)
@@ -459,32 +459,31 @@ class _KeyedDropout(Function):
     any order), and dy itself for the residual."""
 
     @staticmethod
-    def forward(ctx, x, residual, keep, scale, key):
-        ctx.keep, ctx.scale, ctx.key = keep, scale, key
-        return _dropout_raw(x, keep, scale, key, residual)
+    def forward(ctx, x, residual, mask):
+        ctx.mask = mask
+        return _dropout_raw(x, mask, residual)
 
     @staticmethod
     def backward(ctx, gy):
+        need_x, need_residual, _ = ctx.needs_input_grad
         gx = None
-        if ctx.needs_input_grad[0]:
-            if torch.is_grad_enabled():
-                gx = _KeyedDropout.apply(gy, None, ctx.keep, ctx.scale, ctx.key)
-            else:
-                gx = _dropout_raw(gy, ctx.keep, ctx.scale, ctx.key)
-        return gx, (gy if ctx.needs_input_grad[1] else None), None, None, None
+        if need_x and ctx.mask[0] == 1.0:  # p = 0: every element kept, scaled by 1
+            gx = gy
+        elif need_x:
+            gx = _KeyedDropout.apply(gy, None, ctx.mask) if torch.is_grad_enabled() else _dropout_raw(gy, ctx.mask)
+        return gx, (gy if need_residual else None), None
 
 
-def _dropout_raw(x: torch.Tensor, keep: float, scale: float, key,
-                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    code = _element_code(x, "dropout")
+def _dropout_raw(x: torch.Tensor, mask: tuple, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mask: (keep, scale, seed, tag, counter), the entry point's arguments."""
     xr, rows, cols, ldx = _rows_of(x, "dropout")
-    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rr, ldr = None, 0
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    at, ldr = 0, 0
     if residual is not None:
-        rr, _, _, ldr = _rows_of(residual, "dropout residual")
-    seed, tag, counter = key if key is not None else (0, 0, 0)
-    _call_on(x, "lds_dropout_add", xr.data_ptr(), ldx, nat.ptr(rr), ldr, y.data_ptr(), cols, rows, cols, code, keep,
-             scale, seed, tag, counter)
+        residual, _, _, ldr = _rows_of(residual, "dropout residual")
+        at = residual.data_ptr()
+    _call_on(x, "lds_dropout_add", xr.data_ptr(), ldx, at, ldr, y.data_ptr(), cols, rows, cols,
+             nat.ELEMENT_CODES[x.dtype], *mask)
     return y
 
 
@@ -503,9 +502,11 @@ def keyed_dropout(x: torch.Tensor, p: float, key, residual: Optional[torch.Tenso
                                  residual.device != x.device):
         raise ValueError(f"ldsgnn dropout: the residual must match x ({tuple(x.shape)}, {x.dtype}, {x.device}), got "
                          f"{tuple(residual.shape)}, {residual.dtype}, {residual.device}")
+    seed, tag, counter = key if key is not None else (0, 0, 0)
+    mask = (keep, scale, seed, tag, counter)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _KeyedDropout.apply(x, residual, keep, scale, key)
-    return _dropout_raw(x, keep, scale, key, residual)
+        return _KeyedDropout.apply(x, residual, mask)
+    return _dropout_raw(x, mask, residual)
 
 
 # ---------------------------------------------------------------------------
@@ -517,10 +518,11 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
 
 class _NormPlan:
     """The constants of one group_norm_act call."""
-    __slots__ = ("groups", "act", "eps", "keep", "scale", "key")
+    __slots__ = ("groups", "act", "eps", "keep", "mask")
 
     def __init__(self, groups, act, eps, keep, scale, key):
-        self.groups, self.act, self.eps, self.keep, self.scale, self.key = groups, act, eps, keep, scale, key
+        self.groups, self.act, self.eps, self.keep = groups, act, eps, keep
+        self.mask = (keep, scale, *(key if key is not None else (0, 0, 0)))
 
 
 def _samples_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int]:
@@ -544,31 +546,30 @@ def _samples_of(t: torch.Tensor) -> Tuple[torch.Tensor, int, int, int, int]:
 
 
 def _norm_forward(x, weight, bias, pl: _NormPlan):
-    code = _element_code(x, "group_norm_act")
+    code = nat.ELEMENT_CODES[x.dtype]
     xr, samples, n, sx, ldx = _samples_of(x)
     c = x.size(-1)
     dev = x.device
-    y = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((2, samples, pl.groups), dtype=torch.float32, device=dev)
     if x.numel() == 0:
         return y, stats
     pcode = 0 if weight is None and bias is None else nat.ELEMENT_CODES[(bias if weight is None else weight).dtype]
     size = nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 0)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    seed, tag, counter = pl.key if pl.key is not None else (0, 0, 0)
     at = stats.data_ptr()
     _call_on(x, "lds_group_norm_forward", xr.data_ptr(), sx, ldx, samples, n, c, pl.groups, code, nat.ptr(weight),
-             nat.ptr(bias), pcode, pl.eps, pl.act, pl.keep, pl.scale, seed, tag, counter, y.data_ptr(), at,
-             at + 4 * samples * pl.groups, nat.ptr(ws))
+             nat.ptr(bias), pcode, pl.eps, pl.act, *pl.mask, y.data_ptr(), at, at + 4 * samples * pl.groups,
+             nat.ptr(ws))
     return y, stats
 
 
 def _norm_backward(gy, x, weight, bias, stats, pl: _NormPlan, need):
     """(dx, dweight, dbias); `need`: which of them are wanted."""
-    code = _element_code(x, "group_norm_act")
+    code = nat.ELEMENT_CODES[x.dtype]
     c = x.size(-1)
     dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
     want_w, want_b = need[1] and weight is not None, need[2] and bias is not None
     if x.numel() == 0:
         return (dx, torch.zeros_like(weight) if want_w else None, torch.zeros_like(bias) if want_b else None)
@@ -579,11 +580,10 @@ def _norm_backward(gy, x, weight, bias, stats, pl: _NormPlan, need):
     pcode = 0 if weight is None and bias is None else nat.ELEMENT_CODES[(bias if weight is None else weight).dtype]
     size = nat.lib.lds_group_norm_ws_bytes(samples, n, c, pl.groups, code, 1)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    seed, tag, counter = pl.key if pl.key is not None else (0, 0, 0)
     at = stats.data_ptr()
     _call_on(x, "lds_group_norm_backward", gr.data_ptr(), sg, ldg, xr.data_ptr(), sx, ldx, samples, n, c, pl.groups,
-             code, nat.ptr(weight), nat.ptr(bias), pcode, pl.act, pl.keep, pl.scale, seed, tag, counter, at,
-             at + 4 * samples * pl.groups, nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(ws))
+             code, nat.ptr(weight), nat.ptr(bias), pcode, pl.act, *pl.mask, at, at + 4 * samples * pl.groups,
+             nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(ws))
     if pcode:  # 16-bit parameters: one rounding of the fp32 sums
         dw = dw if dw is None else dw.to(weight.dtype)
         db = db if db is None else db.to(bias.dtype)
@@ -641,7 +641,7 @@ class _GroupNormActGrad(Function):
         gy, x, weight, bias = inputs
         mask = None
         if pl.keep < 1.0:
-            mask = _dropout_raw(torch.ones(x.shape, dtype=torch.float32, device=x.device), pl.keep, pl.scale, pl.key)
+            mask = _dropout_raw(torch.ones(x.shape, dtype=torch.float32, device=x.device), pl.mask)
         with torch.enable_grad():
             y = _norm_composed(x, weight, bias, mask, pl)
             wrt = [t for t, k in zip((x, weight, bias), need) if k and t is not None]

@@ -125,6 +125,26 @@ def test_dropout_gradients(device, ops, dtype):
     assert torch.equal(g2.cpu(), plain_dropout(dy, KEY, 0.25))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_dropout_gradients_without_a_mask(device, ops, dtype):
+    """p = 0: dx = dres = dy, at both orders, and each leaf's gradient has memory
+    of its own (adding to one leaves the other and dy as they were)."""
+    g = torch.Generator().manual_seed(10)
+    x, r, dy = (torch.randn(13, 9, generator=g).to(dtype).to(device) for _ in range(3))
+    x.requires_grad_(), r.requires_grad_()
+    y = ops.keyed_dropout(x, 0.0, None, residual=r)
+    assert torch.equal(y, (x.float() + r.float()).to(dtype))
+    given = dy.clone()
+    y.backward(dy)
+    assert torch.equal(x.grad, given) and torch.equal(r.grad, given)
+    x.grad.add_(1.0)
+    assert torch.equal(r.grad, given) and torch.equal(dy, given)
+    w = dy.clone().requires_grad_()
+    (g1,) = torch.autograd.grad(ops.keyed_dropout(x, 0.0, None), x, w, create_graph=True)
+    (g2,) = torch.autograd.grad(g1, w, given)
+    assert torch.equal(g1, given) and torch.equal(g2, given)
+
+
 def test_dropout_entries_at_the_ends(device):
     """lds_dropout and lds_dropout_add take the scale at its word: keep 1 scales
     every element, keep 0 leaves none; lds_dropout takes any keep."""
