@@ -12,14 +12,20 @@ namespace lds {
 
 // y = residual + mask(x), one thread per row quad and 16 bytes of a row: the
 // quad shares its Philox calls, the four rows' loads are independent.  Rows
-// start anywhere (the vectors carry the element's alignment); only a row's last
-// partial vector goes element by element.  Bound by memory: 160000 x 512 bf16 with
-// a residual 98 us (5.0 TB/s, the rate of a large copy), 2708 x 1433 fp32 6.4 us.
-template <typename T, int V, bool RES, bool DROP>
+// start anywhere (the vectors carry the element's alignment).  A row's last
+// vector ends with the row, so that every load is whole; what it has in common
+// with the one before is the same value in both, and both store it (`whole`),
+// unless y overlaps an input: then each stores its own elements only.
+// PAST: the inputs are read past the caches (launch_dropout says when).
+// No lane branches before its loads, so all of them are in flight at once; with
+// the last vector element by element instead, 40000 x 512 of fp16 took 28 us and
+// x 511 74, now 22 and 22.  Bound by memory: 160000 x 512 bf16 with a residual
+// 75 us (6.5 TB/s), 20000 x 257 fp16 9.1, 2708 x 1433 fp32 6.4.
+template <typename T, int V, bool RES, bool DROP, bool PAST>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ x, int64_t ldx,
-                                                          const T* __restrict__ res, int64_t ldr,
-                                                          T* __restrict__ y, int64_t ldy, int64_t rows, int cols,
-                                                          int cvecs, int64_t total, DropKey key) {
+                                                          const T* __restrict__ res, int64_t ldr, T* y, int64_t ldy,
+                                                          int64_t rows, int cols, int cvecs, int64_t total,
+                                                          int whole, DropKey key) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= total) return;
     int64_t rq;
@@ -28,16 +34,14 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ 
     } else {
         rq = t / cvecs;
     }
-    const int j = (int)(t - rq * cvecs) * V;
-    const int w = cols - j;
+    const int j0 = (int)(t - rq * cvecs) * V, j = min(j0, cols - V);
     const int64_t i0 = rq * 4;
-    float v[4][V], a[4][V];
+    Raw<T, V> v[4], a[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        if (i0 + r < rows) {
-            load_part<T, V>(x + (i0 + r) * ldx + j, w, v[r]);
-            if constexpr (RES) load_part<T, V>(res + (i0 + r) * ldr + j, w, a[r]);
-        }
+        const int64_t i = min(i0 + r, rows - 1);  // rows behind the last repeat it
+        v[r] = load_raw<T, V, PAST>(x + i * ldx + j);
+        if constexpr (RES) a[r] = load_raw<T, V, PAST>(res + i * ldr + j);
     }
     bool kept[4][V];
     if constexpr (DROP) {
@@ -48,15 +52,60 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if (i0 + r >= rows) break;
+        float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            float o = v[r][e] * key.scale;
-            if constexpr (DROP) o = kept[r][e] ? o : 0.f;
-            if constexpr (RES) o = o + a[r][e];
-            v[r][e] = o;
+            o[e] = elem<T, V>(v[r], e) * key.scale;
+            if constexpr (DROP) o[e] = kept[r][e] ? o[e] : 0.f;
+            if constexpr (RES) o[e] = o[e] + elem<T, V>(a[r], e);
         }
-        store_part<T, V>(y + (i0 + r) * ldy + j, w, v[r]);
+        T* to = y + (i0 + r) * ldy + j;
+        if (whole || j == j0) {
+            store_vec<T, V>(to, o);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (j + e >= j0) to[e] = (T)o[e];
+        }
     }
+}
+
+// A rows x cols block of stride ld: the bytes from its first element to its last.
+struct Span {
+    uintptr_t lo, hi;
+    Span(const void* p, int64_t rows, int64_t ld, int cols, size_t size)
+        : lo((uintptr_t)p), hi(lo + (uintptr_t)((rows - 1) * ld + cols) * size) {}
+    bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+template <typename T, int V>
+int launch_dropout(const T* x, int64_t ldx, const T* residual, int64_t ldr, T* y, int64_t ldy, int64_t rows, int cols,
+                   bool drop, const DropKey& key, hipStream_t stream) {
+    const int cvecs = (cols - 1) / V + 1;
+    const int64_t total = (rows + 3) / 4 * cvecs;
+    const int64_t blocks = (total + 255) / 256;
+    LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
+    const Span to(y, rows, ldy, cols, sizeof(T));
+    const bool whole = !to.meets(Span(x, rows, ldx, cols, sizeof(T))) &&
+                       !(residual && to.meets(Span(residual, rows, ldr, cols, sizeof(T))));
+    // Operands that fill the memory-side cache leave it to the result, which the
+    // next call reads.  Past it and through it, in us, alone / with a multiplication
+    // of the result after it: 160000 x 512 bf16 75 / 121 and 88 / 129, 130000 x 512
+    // fp32 118 / 190 and 141 / 239, 200000 x 256 bf16 (307 MB) 50 / 79 and 50 / 77;
+    // below the cache's size the inputs may lie in it (160000 x 256, 246 MB, read
+    // past it: +1 %).
+    const int64_t bytes = rows * cols * (int64_t)sizeof(T);
+    const bool past = (residual ? 3 : 2) * bytes > kMemorySideCache;
+    const auto go = [&](auto res, auto dr, auto ps) {
+        hipLaunchKernelGGL((dropout_add_kernel<T, V, decltype(res)::value, decltype(dr)::value, decltype(ps)::value>),
+                           dim3((unsigned)blocks), dim3(256), 0, stream, x, ldx, residual, ldr, y, ldy, rows, cols,
+                           cvecs, total, (int)whole, key);
+    };
+    const auto with = [](bool b, auto&& f) { b ? f(BoolC<true>{}) : f(BoolC<false>{}); };
+    with(residual != nullptr, [&](auto res) {
+        with(drop, [&](auto dr) { with(past, [&](auto ps) { go(res, dr, ps); }); });
+    });
+    LDS_RETURN_LAST_ERROR();
 }
 
 }  // namespace lds
@@ -83,21 +132,11 @@ extern "C" int lds_dropout_add(const void* x, int64_t ldx, const void* residual,
         constexpr int V = 16 / (int)sizeof(T);
         DropKey key;
         const bool drop = drop_key(keep_prob, scale, seed, tag, counter, &key);
-        const int cvecs = (cols - 1) / V + 1;
-        const int64_t total = (rows + 3) / 4 * cvecs;
-        const int64_t blocks = (total + 255) / 256;
-        LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
-        auto go = [&](auto res, auto dr) {
-            hipLaunchKernelGGL((dropout_add_kernel<T, V, decltype(res)::value, decltype(dr)::value>),
-                               dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, (const T*)x, ldx,
-                               (const T*)residual, ldr, (T*)y, ldy, rows, cols, cvecs, total, key);
-        };
-        if (residual) {
-            drop ? go(BoolC<true>{}, BoolC<true>{}) : go(BoolC<true>{}, BoolC<false>{});
-        } else {
-            drop ? go(BoolC<false>{}, BoolC<true>{}) : go(BoolC<false>{}, BoolC<false>{});
-        }
-        LDS_RETURN_LAST_ERROR();
+        const auto* xs = (const T*)x;
+        const auto* rs = (const T*)residual;
+        if (cols < V)  // rows shorter than a vector: single columns
+            return launch_dropout<T, 1>(xs, ldx, rs, ldr, (T*)y, ldy, rows, cols, drop, key, (hipStream_t)stream);
+        return launch_dropout<T, V>(xs, ldx, rs, ldr, (T*)y, ldy, rows, cols, drop, key, (hipStream_t)stream);
     });
 }
 

@@ -14,6 +14,9 @@ namespace lds {
 using bf16_t = __bf16;
 using f16_t = _Float16;
 
+// The cache between the memory and the chip's L2s.
+constexpr int64_t kMemorySideCache = (int64_t)256 << 20;
+
 // V consecutive elements as one load or store.  Rows of an odd length start at
 // any multiple of the element size: the type carries the element's alignment,
 // and gfx950's global memory takes a 16-byte access at any address.
@@ -80,9 +83,13 @@ __device__ __forceinline__ float load_param(const void* p, int code, int64_t i) 
 // V consecutive elements as they lie in memory, and as fp32.
 template <typename T, int V>
 using Raw = typename VecOf<T, V>::type;
-template <typename T, int V>
+// PAST: a last read, which leaves the caches to others.
+template <typename T, int V, bool PAST = false>
 __device__ __forceinline__ Raw<T, V> load_raw(const T* __restrict__ p) {
-    return *reinterpret_cast<const Raw<T, V>*>(p);
+    if constexpr (PAST)
+        return __builtin_nontemporal_load(reinterpret_cast<const Raw<T, V>*>(p));
+    else
+        return *reinterpret_cast<const Raw<T, V>*>(p);
 }
 template <typename T, int V>
 __device__ __forceinline__ float elem(const Raw<T, V>& v, int e) {

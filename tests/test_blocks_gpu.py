@@ -125,6 +125,38 @@ def test_dropout_gradients(device, ops, dtype):
     assert torch.equal(g2.cpu(), plain_dropout(dy, KEY, 0.25))
 
 
+def test_dropout_of_operands_that_fill_the_cache(device, ops):
+    """Three operands of 96 MB are read past the memory-side cache, two are not:
+    in fp32 the residual's sum is one IEEE operation, so both have the same bits."""
+    g = torch.Generator(device=device).manual_seed(12)
+    x, r = (torch.randn(46003, 521, generator=g, device=device) for _ in range(2))
+    both = ops.keyed_dropout(x, 0.3, KEY, residual=r)
+    alone = ops.keyed_dropout(x, 0.3, KEY)
+    assert torch.equal(both, alone + r)
+    assert torch.equal(alone[:64].cpu(), plain_dropout(x[:64].cpu(), KEY, 0.3))
+    assert torch.equal(ops.keyed_dropout(x, 0.0, None, residual=r), x + r)
+
+
+@pytest.mark.parametrize("cols", [1, 3, 4, 5, 7, 8, 257])
+def test_dropout_in_place(device, cols):
+    """lds_dropout over its own input, and into a block that begins inside it:
+    what two threads read of a row's last vector is not what the other wrote."""
+    from ldsgnn import _native as nat
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(1031, cols, generator=g)
+    want = plain_dropout(x, KEY, 0.5)
+    y = x.to(device)
+    nat.call("lds_dropout", y.data_ptr(), cols, y.data_ptr(), cols, 1031, cols, 0.5, 2.0, *KEY, nat.stream_of(y.device))
+    assert torch.equal(y.cpu(), want)
+    wide = torch.full((1031, 2 * cols + 1), 7.0)  # input and result side by side in one block's rows
+    wide[:, :cols] = x
+    wide = wide.to(device)
+    nat.call("lds_dropout", wide.data_ptr(), 2 * cols + 1, wide.data_ptr() + 4 * (cols + 1), 2 * cols + 1, 1031, cols,
+             0.5, 2.0, *KEY, nat.stream_of(wide.device))
+    assert torch.equal(wide[:, cols + 1:].cpu(), want) and torch.equal(wide[:, :cols].cpu(), x)
+    assert (wide[:, cols] == 7.0).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_dropout_gradients_without_a_mask(device, ops, dtype):
     """p = 0: dx = dres = dy, at both orders, and each leaf's gradient has memory
