@@ -112,13 +112,14 @@ template <typename T, int V>
 struct Quad {
     Raw<T, V> row[4];
 
+    template <bool PAST = false>
     __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, const NormPlace& p, int64_t q,
                                          const QuadRows& in) {
         const T* at = base + (4 * q - p.f0) * ld;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = r < in.lo ? in.lo : r >= in.hi ? in.hi - 1 : r;
-            row[r] = load_raw<T, V>(at + k * ld);
+            row[r] = load_raw<T, V, PAST>(at + k * ld);
         }
     }
 };
@@ -294,7 +295,7 @@ struct NormParams {
 };
 
 // A thread's vector of a row; at a row's end across groups only what it owns.
-template <typename T, int V, bool SPAN>
+template <typename T, int V, bool SPAN, bool PAST = false>
 __device__ __forceinline__ void store_own(T* __restrict__ at, int skip, const float (&o)[V]) {
     if constexpr (SPAN) {
         if (skip) {
@@ -304,7 +305,7 @@ __device__ __forceinline__ void store_own(T* __restrict__ at, int skip, const fl
             return;
         }
     }
-    store_vec<T, V>(at, o);
+    store_vec<T, V, PAST>(at, o);
 }
 
 // Calls f with an integral constant for the activation / the vector width.
@@ -324,6 +325,17 @@ inline int with_vec(int v, bool span, F&& f) {
     if (v == 2) return f(IntC<2>{}, BoolC<false>{});
     return f(IntC<1>{}, BoolC<false>{});
 }
+
+// A second pass's reads are the last of x and dy, and a result of half the
+// memory-side cache does not stay there until it is read: both may go past the
+// caches, where a wave's vectors cover whole 128-byte lines (with parts of lines a
+// line is fetched again for each: 8 x 20000 x 25 groups of 4 fp16 44.6 -> 49.2 us).
+inline bool whole_lines(const void* p, int64_t samples, int64_t stride, int64_t ld, int c, int size) {
+    const int64_t line = 128;
+    return (uintptr_t)p % line == 0 && ld * size % line == 0 && (int64_t)c * size % line == 0 &&
+           (samples == 1 || stride * size % line == 0);
+}
+inline bool past_caches(int64_t result_bytes) { return result_bytes > kMemorySideCache / 2; }
 
 // ... for a slab thread's quads: at most 32 values of x are held.
 template <int V, typename F>

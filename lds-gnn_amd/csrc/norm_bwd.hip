@@ -43,6 +43,7 @@ struct BackQuad {
         }
     }
     // dx = (γ rstd scale) h + (-(rstd² m2) (x - mean) - rstd m1)
+    template <bool PAST>
     __device__ __forceinline__ void store(const QuadRows& in, const float (&rws)[V], const GroupValue<V, SPAN>& k0,
                                           const GroupValue<V, SPAN>& k1, T* __restrict__ at, int64_t ld,
                                           int skip) const {
@@ -52,7 +53,7 @@ struct BackQuad {
             float o[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) o[e] = __builtin_fmaf(rws[e], h[r][e], __builtin_fmaf(k1[e], d[r][e], k0[e]));
-            store_own<T, V, SPAN>(at + r * ld, skip, o);
+            store_own<T, V, SPAN, PAST>(at + r * ld, skip, o);
         }
     }
 };
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
         float rws[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) rws[e] = Q > 1 ? par.rw[e] * scale : par.rw[e];
-        b.store(quad_rows(p, q), rws, k0, k1, ds + 4 * q * a.c, a.c, 0);
+        b.template store<false>(quad_rows(p, q), rws, k0, k1, ds + 4 * q * a.c, a.c, 0);
     }
 }
 
@@ -319,7 +320,8 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
     }
 }
 
-template <typename T, int V, int ACT, bool DROP, bool SPAN>
+// PAST: x and dy are read past the caches (1), dx is stored past them too (2).
+template <typename T, int V, int ACT, bool DROP, bool SPAN, int PAST>
 __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __restrict__ dy, int64_t sdy, int64_t lddy,
                                                                  const T* __restrict__ x, NormArgs a,
                                                                  const float* __restrict__ mean,
@@ -350,15 +352,15 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __rest
     each_quad_ahead<QuadPair<T, V>>(
         a, p,
         [&](QuadPair<T, V>& d, int64_t q, const QuadRows in) {
-            d.x.load(xs, a.ldx, p, q, in);
-            d.g.load(gs, lddy, p, q, in);
+            d.x.template load<(PAST > 0)>(xs, a.ldx, p, q, in);
+            d.g.template load<(PAST > 0)>(gs, lddy, p, q, in);
         },
         [&](const QuadPair<T, V>& d, int64_t q, const QuadRows in) {
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
         BackQuad<T, V, ACT, DROP, SPAN> b;
         b.eval(d.x, d.g, par, mu, kept);
-        b.store(in, rws, k0, k1, ds + 4 * q * a.c, a.c, p.skip);
+        b.template store<(PAST > 1)>(in, rws, k0, k1, ds + 4 * q * a.c, a.c, p.skip);
     });
 }
 
@@ -397,11 +399,15 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && cblocks < (int64_t)1 << 31);
     float2* sums = (float2*)ws;
     float2* means = k.slab ? nullptr : sums + samples * a.parts * (int64_t)c;
+    const int size = norm_elem(dtype);
+    const bool lines = whole_lines(x, samples, sx, ldx, c, size) && whole_lines(dy, samples, sdy, lddy, c, size) &&
+                       whole_lines(dx, 1, 0, c, c, size);
+    const int past = !lines ? 0 : past_caches(samples * n * c * size) ? 2 : 1;
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
         return with_vec<16 / (int)sizeof(T)>(k.v, a.span, [&](auto vc, auto sc) -> int {
             constexpr int V = decltype(vc)::value;
-            constexpr bool SPAN = decltype(sc)::value;
+            constexpr bool SPAN = decltype(sc)::value, WIDE = !SPAN && V * sizeof(T) == 16;
             return with_act(act, [&](auto ac) -> int {
                 constexpr int ACT = decltype(ac)::value;
                 auto go = [&](auto dr) {
@@ -422,10 +428,12 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
                     if (cblocks)
                         hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3((unsigned)cblocks), dim3(kNormThreads), 0, st,
                                            (const float2*)sums, a, pairs, means, dweight, dbias);
-                    if (!k.slab && dx)
-                        hipLaunchKernelGGL((gn_bwd_dx_kernel<T, V, ACT, DROP, SPAN>), dim3((unsigned)blocks),
-                                           dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
-                                           rstd, (const float2*)means, (T*)dx);
+                    auto second = [&](auto ps) {
+                        hipLaunchKernelGGL((gn_bwd_dx_kernel<T, V, ACT, DROP, SPAN, WIDE ? decltype(ps)::value : 0>),
+                                           dim3((unsigned)blocks), dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy,
+                                           (const T*)x, a, mean, rstd, (const float2*)means, (T*)dx);
+                    };
+                    if (!k.slab && dx) past == 2 ? second(IntC<2>{}) : past ? second(IntC<1>{}) : second(IntC<0>{});
                 };
                 drop ? go(BoolC<true>{}) : go(BoolC<false>{});
                 LDS_RETURN_LAST_ERROR();

@@ -10,7 +10,7 @@ struct Moments {
 };
 
 // y of a quad from x.
-template <typename T, int V, int ACT, bool DROP, bool SPAN>
+template <typename T, int V, int ACT, bool DROP, bool SPAN, bool PAST = false>
 __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& in, const NormParams<V>& par,
                                            const GroupValue<V, SPAN>& mu, const bool (&kept)[4][V], float scale,
                                            T* __restrict__ at, int64_t ld, int skip) {
@@ -24,7 +24,7 @@ __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& 
             o[e] = act_f<ACT>(z);
             if constexpr (DROP) o[e] = kept[r][e] ? o[e] * scale : 0.f;
         }
-        store_own<T, V, SPAN>(at + r * ld, skip, o);
+        store_own<T, V, SPAN, PAST>(at + r * ld, skip, o);
     }
 }
 
@@ -304,7 +304,8 @@ __global__ __launch_bounds__(kNormThreads) void gn_combine_kernel(const Moments*
     }
 }
 
-template <typename T, int V, int ACT, bool DROP, bool SPAN>
+// PAST: x is read and y stored past the caches.
+template <typename T, int V, int ACT, bool DROP, bool SPAN, bool PAST>
 __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restrict__ x, NormArgs a,
                                                                 const float* __restrict__ mean,
                                                                 const float* __restrict__ rstd, T* __restrict__ y) {
@@ -322,10 +323,10 @@ __global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restr
     par.times(rs);
     each_quad(a, p, [&](int64_t q, const QuadRows in) {
         Quad<T, V> v;
-        v.load(xs, a.ldx, p, q, in);
+        v.template load<PAST>(xs, a.ldx, p, q, in);
         bool kept[4][V];
         if constexpr (DROP) columns.quad(a.key, (uint32_t)q, kept);
-        apply_quad<T, V, ACT, DROP, SPAN>(v, in, par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c, p.skip);
+        apply_quad<T, V, ACT, DROP, SPAN, PAST>(v, in, par, mu, kept, a.key.scale, ys + 4 * q * a.c, a.c, p.skip);
     });
 }
 
@@ -370,11 +371,14 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     const int64_t pairs = samples * groups;
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && samples * b.parts * b.chunks < (int64_t)1 << 31);
     LDS_CHECK_ARG(pairs < (int64_t)1 << 32);
+    const int size = norm_elem(dtype);
+    const bool past = past_caches(samples * n * c * size) && whole_lines(x, samples, sx, ldx, c, size) &&
+                      whole_lines(y, 1, 0, c, c, size);
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);
         return with_vec<16 / (int)sizeof(T)>(k.v, a.span, [&](auto vc, auto sc) -> int {
             constexpr int V = decltype(vc)::value;
-            constexpr bool SPAN = decltype(sc)::value;
+            constexpr bool SPAN = decltype(sc)::value, WIDE = !SPAN && V * sizeof(T) == 16;
             if (!k.slab) {
                 if constexpr (SPAN)
                     hipLaunchKernelGGL((gn_stats_span_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0,
@@ -394,10 +398,13 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
                                            dim3((unsigned)blocks), dim3(k.threads), 0, st, (const T*)x, a, eps, (T*)y,
                                            mean, rstd);
                     };
-                    if (!k.slab)
-                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP, SPAN>),
+                    auto apply = [&](auto ps) {
+                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP, SPAN, WIDE && decltype(ps)::value>),
                                            dim3((unsigned)(samples * b.parts * b.chunks)), dim3(kNormThreads), 0, st,
                                            (const T*)x, b, mean, rstd, (T*)y);
+                    };
+                    if (!k.slab)
+                        past ? apply(BoolC<true>{}) : apply(BoolC<false>{});
                     else if constexpr (!SPAN)
                         with_quads<V>(k.quads, slab);
                 };

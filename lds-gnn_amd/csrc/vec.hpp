@@ -40,7 +40,8 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[V])
     }
 }
 
-template <typename T, int V>
+// PAST: a store that leaves the caches to others.
+template <typename T, int V, bool PAST = false>
 __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V]) {
     if constexpr (V == 1) {
         p[0] = (T)f[0];
@@ -48,7 +49,10 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V]
         typename VecOf<T, V>::type v;
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = (T)f[e];
-        *reinterpret_cast<typename VecOf<T, V>::type*>(p) = v;
+        if constexpr (PAST)
+            __builtin_nontemporal_store(v, reinterpret_cast<typename VecOf<T, V>::type*>(p));
+        else
+            *reinterpret_cast<typename VecOf<T, V>::type*>(p) = v;
     }
 }
 
