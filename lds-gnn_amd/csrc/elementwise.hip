@@ -70,14 +70,6 @@ __global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ 
     }
 }
 
-// A rows x cols block of stride ld: the bytes from its first element to its last.
-struct Span {
-    uintptr_t lo, hi;
-    Span(const void* p, int64_t rows, int64_t ld, int cols, size_t size)
-        : lo((uintptr_t)p), hi(lo + (uintptr_t)((rows - 1) * ld + cols) * size) {}
-    bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
-};
-
 template <typename T, int V>
 int launch_dropout(const T* x, int64_t ldx, const T* residual, int64_t ldr, T* y, int64_t ldy, int64_t rows, int cols,
                    bool drop, const DropKey& key, hipStream_t stream) {
@@ -85,9 +77,9 @@ int launch_dropout(const T* x, int64_t ldx, const T* residual, int64_t ldr, T* y
     const int64_t total = (rows + 3) / 4 * cvecs;
     const int64_t blocks = (total + 255) / 256;
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
-    const Span to(y, rows, ldy, cols, sizeof(T));
-    const bool whole = !to.meets(Span(x, rows, ldx, cols, sizeof(T))) &&
-                       !(residual && to.meets(Span(residual, rows, ldr, cols, sizeof(T))));
+    const auto span = [&](const T* p, int64_t ld) { return ByteSpan(p, (rows - 1) * ld + cols, sizeof(T)); };
+    const ByteSpan to = span(y, ldy);
+    const bool whole = !to.meets(span(x, ldx)) && !(residual && to.meets(span(residual, ldr)));
     // Operands that fill the memory-side cache leave it to the result, which the
     // next call reads.  Past it and through it, in us, alone / with a multiplication
     // of the result after it: 160000 x 512 bf16 75 / 121 and 88 / 129, 130000 x 512

@@ -392,6 +392,9 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
     a.weight = weight;
     a.bias = bias;
     a.ptype = ptype;
+    const int size = norm_elem(dtype);
+    a.whole = dx && whole_store(dx, samples, n, c, size, x, sx, ldx) &&
+              whole_store(dx, samples, n, c, size, dy, sdy, lddy);
     const int64_t blocks = k.slab ? slab_blocks(a) : samples * a.parts * a.chunks;
     const int64_t pairs = dx && !k.slab ? samples * groups : 0;
     const bool params = dweight || dbias;
@@ -399,7 +402,6 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && cblocks < (int64_t)1 << 31);
     float2* sums = (float2*)ws;
     float2* means = k.slab ? nullptr : sums + samples * a.parts * (int64_t)c;
-    const int size = norm_elem(dtype);
     const bool lines = whole_lines(x, samples, sx, ldx, c, size) && whole_lines(dy, samples, sdy, lddy, c, size) &&
                        whole_lines(dx, 1, 0, c, c, size);
     const int past = !lines ? 0 : past_caches(samples * n * c * size) ? 2 : 1;

@@ -361,6 +361,8 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     a.weight = weight;
     a.bias = bias;
     a.ptype = ptype;
+    const int size = norm_elem(dtype);
+    a.whole = whole_store(y, samples, n, c, size, x, sx, ldx);
     NormArgs b = a;  // the second pass of the parts form
     if (!k.slab) {
         const NormArgs cut = norm_plan(samples, n, c, groups, dtype, kForwardSlabThreads, kApplyBlocks).a;
@@ -371,7 +373,6 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     const int64_t pairs = samples * groups;
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && samples * b.parts * b.chunks < (int64_t)1 << 31);
     LDS_CHECK_ARG(pairs < (int64_t)1 << 32);
-    const int size = norm_elem(dtype);
     const bool past = past_caches(samples * n * c * size) && whole_lines(x, samples, sx, ldx, c, size) &&
                       whole_lines(y, 1, 0, c, c, size);
     return with_type(dtype, [&](auto zero) -> int {

@@ -17,6 +17,14 @@ using f16_t = _Float16;
 // The cache between the memory and the chip's L2s.
 constexpr int64_t kMemorySideCache = (int64_t)256 << 20;
 
+// The bytes from a block's first element to its last.
+struct ByteSpan {
+    uintptr_t lo, hi;
+    ByteSpan(const void* p, int64_t elements, size_t size)
+        : lo((uintptr_t)p), hi(lo + (uintptr_t)elements * size) {}
+    bool meets(const ByteSpan& o) const { return lo < o.hi && o.lo < hi; }
+};
+
 // V consecutive elements as one load or store.  Rows of an odd length start at
 // any multiple of the element size: the type carries the element's alignment,
 // and gfx950's global memory takes a 16-byte access at any address.

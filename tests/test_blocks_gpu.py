@@ -728,6 +728,36 @@ def test_side_stream_runs_the_same_bits(device, ops):
     assert all(torch.equal(a, b) for a, b in zip(ref, got))
 
 
+@pytest.mark.parametrize("n,groups,cg", [(5000, 12, 5), (5000, 7, 5), (5000, 4, 8), (60, 7, 5)])
+def test_group_norm_entries_in_place(device, n, groups, cg):
+    """y over x and dx over dy: the bits of separate results, also where a row's
+    last vector shares elements with the one before it."""
+    from ldsgnn import _native as nat
+    c, half = groups * cg, nat.ELEMENT_CODES[torch.float16]
+    g = torch.Generator().manual_seed(n + c)
+    x, dy = (torch.randn(3, n, c, generator=g).half().to(device) for _ in range(2))
+    stats = torch.empty(2, 3, groups, device=device)
+    at, to = stats.data_ptr(), stats.data_ptr() + 4 * 3 * groups
+    ws = torch.empty(max(nat.lib.lds_group_norm_ws_bytes(3, n, c, groups, half, k) for k in (0, 1)) + 16,
+                     dtype=torch.uint8, device=device)
+
+    def forward(a, y):
+        nat.call("lds_group_norm_forward", a.data_ptr(), n * c, c, 3, n, c, groups, half, 0, 0, 0, 1e-5, 2, 0.75,
+                 4.0 / 3.0, *KEY, y.data_ptr(), at, to, ws.data_ptr(), nat.stream_of(a.device))
+        return y
+
+    def backward(d, dx):
+        nat.call("lds_group_norm_backward", d.data_ptr(), n * c, c, x.data_ptr(), n * c, c, 3, n, c, groups, half, 0, 0,
+                 0, 2, 0.75, 4.0 / 3.0, *KEY, at, to, dx.data_ptr(), 0, 0, ws.data_ptr(), nat.stream_of(x.device))
+        return dx
+
+    y, dx = forward(x, torch.empty_like(x)), backward(dy, torch.empty_like(x))
+    here = dy.clone()
+    assert torch.equal(backward(here, here), dx)
+    here = x.clone()
+    assert torch.equal(forward(here, here), y)
+
+
 def test_captured_run_replays_the_eager_bits(device, ops):
     """Forward, backward and the 8-bit product in one captured graph, replayed
     with new inputs and eager work in between; kernel nodes only."""
