@@ -1062,14 +1062,17 @@ class LdsEngine:
         nb = (self.n + 127) // 128
         return form == "bf16x3-direct" or (form == "bf16x3" and nb * (nb + 1) // 2 <= 256)
 
+    def _alloc_planes(self) -> None:
+        if self.Up is None:
+            ne = int(nat.lib.lds_planes_t128_elems(self.n, self.ktot))
+            self.Up = torch.zeros(ne, dtype=torch.int16, device=self.dev)
+            self.Vp = torch.zeros(ne, dtype=torch.int16, device=self.dev)
+
     def _uv(self):
         """(U, V, ld) of the factor producers' launches: fp32 rows (ld > 0) or,
         in a planes window, the split planes (ld = -row tiles)."""
         if self._planes_now:
-            if self.Up is None:
-                ne = int(nat.lib.lds_planes_t128_elems(self.n, self.ktot))
-                self.Up = torch.zeros(ne, dtype=torch.int16, device=self.dev)
-                self.Vp = torch.zeros(ne, dtype=torch.int16, device=self.dev)
+            self._alloc_planes()
             return nat.ptr(self.Up), nat.ptr(self.Vp), -((self.n + 127) // 128)
         return nat.ptr(self.U), nat.ptr(self.V), self.ldu
 
@@ -1661,6 +1664,11 @@ class LdsEngine:
         self.prefetch_draw = bool(prefetch) and \
             self._prefetch_ok(tau, tau * self.kg + HID + self.cw, exchange=grad_reducer is not None, check_flag=False)
         self._enter_window_state(self.prefetch_draw, tau)
+        if self._planes_window(tau, grad_reducer):
+            # cleared here: inside the capture the clearing would be a node of the
+            # first graph alone, and a group replayed before it would read what
+            # the memory held
+            self._alloc_planes()
         s = torch.cuda.Stream(self.dev)
         s.wait_stream(torch.cuda.current_stream(self.dev))
         if capture_exchange is None:

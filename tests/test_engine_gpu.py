@@ -46,6 +46,23 @@ def test_graph_replay_equals_eager(group, windows):
     assert a.scalars_host() == b.scalars_host()
 
 
+def test_window_capture_allocates_no_state():
+    """What a captured window reads and does not write first is allocated (and
+    cleared) before the capture: a clearing inside it would belong to the first
+    of the graphs alone, and a group of windows replayed first would read stale
+    memory."""
+    eng = run_engine_and_oracle(n=130, f_in=30, classes=5, steps=1, tau=5, dropout=0.5, seed=9)["engine"]
+    missing, plain = [], eng._uv
+
+    def uv():
+        if eng._planes_now and torch.cuda.is_current_stream_capturing():
+            missing.append(eng.Up is None)
+        return plain()
+    eng._uv = uv
+    eng.capture_window(5, windows=2)
+    assert missing and not any(missing)
+
+
 def test_batched_window_sampling_equals_stepwise():
     """run_window draws the window's graphs in one batched launch set: same
     draws (counters), same results as sampling step by step."""
