@@ -35,7 +35,9 @@ S = 1 is the reference's single chain.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import gc
 from collections import OrderedDict
 from typing import List, Optional
 
@@ -131,6 +133,20 @@ def _csr_of(dense: torch.Tensor):
             sp.values().to(torch.float32).contiguous())
 
 
+@contextlib.contextmanager
+def _no_collection():
+    """No garbage collection inside: a collected CUDAGraph (an engine's, in a
+    reference cycle) synchronizes the device as it goes, which a capture does
+    not permit, and its destructor ends the process over that."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if on:
+            gc.enable()
+
+
 def capture_into(graph, stream, body, pool=None, error_mode: str = "global", joins=()):
     """Capture body() into `graph` on `stream` (torch.cuda.CUDAGraph
     capture_begin / capture_end).
@@ -143,7 +159,7 @@ def capture_into(graph, stream, body, pool=None, error_mode: str = "global", joi
     error is re-raised.  Without this, torch.cuda.graph's __exit__ raised
     hipErrorStreamCaptureUnjoined on top of the real cause (
     "What's weak" #8) and left the stream capturing."""
-    with torch.cuda.stream(stream):
+    with _no_collection(), torch.cuda.stream(stream):
         if pool is None:
             graph.capture_begin(capture_error_mode=error_mode)
         else:
@@ -1725,7 +1741,7 @@ class LdsEngine:
             tail.capture_begin(pool=pool)
 
         err = None
-        with torch.cuda.stream(s):
+        with _no_collection(), torch.cuda.stream(s):
             head.capture_begin(pool=pool)
             try:
                 self.run_window(tau, grad_reducer=switch)

@@ -119,6 +119,29 @@ def test_successful_capture_ends_once(fake_cuda):
     assert g.calls == [("begin", "global"), "end"]
 
 
+@pytest.mark.parametrize("fails", [False, True])
+def test_no_garbage_collection_inside_a_capture(fake_cuda, fails):
+    import gc
+    main, side = _Stream("capture"), _Stream("side")
+    seen = []
+
+    def body():
+        seen.append(gc.isenabled())
+        if fails:
+            raise RuntimeError("launch")
+
+    assert gc.isenabled()
+    with pytest.raises(RuntimeError) if fails else contextlib.nullcontext():
+        E.capture_into(_Graph(main, side), main, body, joins=(side,))
+    assert seen == [False] and gc.isenabled()
+    gc.disable()  # a caller's own choice stays
+    try:
+        E.capture_into(_Graph(_Stream("a"), side), _Stream("a"), lambda: None)
+        assert not gc.isenabled()
+    finally:
+        gc.enable()
+
+
 def test_capture_status_classes():
     assert E._capture_status(None) == E._CAPTURE_OK
     assert E._capture_status(nat.NativeError("x")) == E._CAPTURE_FATAL
