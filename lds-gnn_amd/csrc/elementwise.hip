@@ -22,10 +22,9 @@ namespace lds {
 // x 511 74, now 22 and 22.  Bound by memory: 160000 x 512 bf16 with a residual
 // 75 us (6.5 TB/s), 20000 x 257 fp16 9.1, 2708 x 1433 fp32 6.4.
 template <typename T, int V, bool RES, bool DROP, bool PAST>
-__global__ __launch_bounds__(256) void dropout_add_kernel(const T* __restrict__ x, int64_t ldx,
-                                                          const T* __restrict__ res, int64_t ldr, T* y, int64_t ldy,
-                                                          int64_t rows, int cols, int cvecs, int64_t total,
-                                                          int whole, DropKey key) {
+__global__ __launch_bounds__(256) void dropout_add_kernel(const T* x, int64_t ldx, const T* res, int64_t ldr,
+                                                          T* y, int64_t ldy, int64_t rows, int cols, int cvecs,
+                                                          int64_t total, int whole, DropKey key) {
     const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (t >= total) return;
     int64_t rq;

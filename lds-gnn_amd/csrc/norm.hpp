@@ -327,10 +327,15 @@ inline int with_vec(int v, bool span, F&& f) {
     return f(IntC<1>{}, BoolC<false>{});
 }
 
-// A second pass's reads are the last of x and dy, and a result of half the
-// memory-side cache does not stay there until it is read: both may go past the
-// caches, where a wave's vectors cover whole 128-byte lines (with parts of lines a
-// line is fetched again for each: 8 x 20000 x 25 groups of 4 fp16 44.6 -> 49.2 us).
+// The backward's second pass reads x and dy for the last time: past the caches, if
+// a wave's vectors cover whole 128-byte lines (8 x 20000 x 256 bf16: both passes 91
+// -> 79 us; with parts of lines, each fetched again, 8 x 20000 x 25 groups of 4 fp16
+// 44.6 -> 49.2).  A result of more than half the memory-side cache goes past it
+// too, with the forward's reads: alone / with a multiplication of the result
+// after it, in us, 16 x 20000 x 256 fp32 forward 206 / 322 -> 171 / 294, backward 339 /
+// 457 -> 288 / 433; bf16 (164 MB) 107 / 141 -> 86 / 142, 186 / 236 -> 144 / 218.  A
+// smaller one is read from the cache afterwards: 8 x 20000 x 256 bf16 (82 MB) would
+// gain 8 of 58 alone and lose 3 of 85 with what follows.
 inline bool whole_lines(const void* p, int64_t samples, int64_t stride, int64_t ld, int c, int size) {
     const int64_t line = 128;
     return (uintptr_t)p % line == 0 && ld * size % line == 0 && (int64_t)c * size % line == 0 &&
