@@ -110,8 +110,8 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
     return v;
 }
 
-// The V values of a row from j on, zeros behind its end: one whole load that ends
-// with the row at most, moved down by what lies before j.  cols >= V.  (Element
+// The V values of a row from j < cols on, zeros behind its end: one whole load that
+// ends with the row at most, moved down by what lies before j.  cols >= V.  (Element
 // by element, 20000 rows of 4095 bf16 took 71 us to quantise, so 49; of 4096 47.)
 template <typename T, int V>
 __device__ __forceinline__ void load_to_end(const T* __restrict__ row, int j, int cols, float (&f)[V]) {
@@ -122,12 +122,12 @@ __device__ __forceinline__ void load_to_end(const T* __restrict__ row, int j, in
     } u;
     const int at = min(j, cols - V);
     u.raw = load_raw<T, V>(row + at);
-    if (const int bits = (j - at) * 8 * (int)sizeof(T)) {
+    if (const int bits = (j - at) * 8 * (int)sizeof(T)) {  // j - at < V: fewer than 128
         if (bits < 64) {
             u.half[0] = u.half[0] >> bits | u.half[1] << (64 - bits);
             u.half[1] >>= bits;
         } else {
-            u.half[0] = bits < 128 ? u.half[1] >> (bits - 64) : 0;
+            u.half[0] = u.half[1] >> (bits - 64);
             u.half[1] = 0;
         }
     }
@@ -198,7 +198,12 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     }
     for (int64_t j = (int64_t)(t + R * G) * V; j < ldq; j += G * V) {
         float f[V];
-        load_to_end<T, V>(xr, (int)j, cols, f);
+        if (j < cols) {
+            load_to_end<T, V>(xr, (int)j, cols, f);
+        } else {  // padding: the row may be shorter than a vector, or empty
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = 0.f;
+        }
         k.put<V>(qr + j, f);
     }
 }

@@ -575,6 +575,53 @@ def test_quantize_rows_borders(device, ops):
     assert torch.equal(q.cpu(), eq)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [0, 1, 3, 5, 7, 9])
+@pytest.mark.parametrize("ldq", [16, 4112, 8208, 12304])
+def test_quantize_entry_pads_any_row(device, dtype, cols, ldq):
+    """Rows shorter than a vector, or empty, in rows of 8 bits of any length:
+    the padding is 0 and nothing but the row is read (x is NULL at cols = 0)."""
+    from ldsgnn import _native as nat
+    g = torch.Generator().manual_seed(cols)
+    x = torch.randn(5, cols, generator=g).to(dtype)
+    xd = x.to(device)
+    q = torch.full((5, ldq), 85, dtype=torch.int8, device=device)
+    scale = torch.full((5,), 7.0, device=device)
+    nat.call("lds_quantize_rows", xd.data_ptr() if cols else 0, cols, 5, cols, nat.ELEMENT_CODES[dtype], q.data_ptr(),
+             ldq, scale.data_ptr(), nat.stream_of(xd.device))
+    eq, es = quantize64(x)
+    assert torch.equal(scale.cpu(), es) and torch.equal(q[:, :cols].cpu(), eq)
+    assert not q[:, cols:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,ldq", [(5, 3, 8208), (5, 7, 4112), (2, 5, 16368), (3, 9, 12304)])
+def test_int8_linear_entry_with_long_rows_in_the_workspace(device, dtype, m, k, ldq):
+    from ldsgnn import _native as nat
+    g = torch.Generator().manual_seed(m + k)
+    x, w = torch.randn(m, k, generator=g).to(dtype), ints(g, 19, k)
+    wq = torch.zeros(19, 16, dtype=torch.int8, device=device)
+    wq[:, :k] = w.to(device)
+    xd, one, y = x.to(device), torch.ones(19, device=device), torch.empty(m, 19, device=device)
+    q, xs = torch.empty(m, ldq, dtype=torch.int8, device=device), torch.empty(m, device=device)
+    nat.call("lds_int8_linear", xd.data_ptr(), k, nat.ELEMENT_CODES[dtype], q.data_ptr(), ldq, xs.data_ptr(),
+             wq.data_ptr(), 16, one.data_ptr(), 0, 0, m, 19, k, y.data_ptr(), 19, 0, nat.stream_of(xd.device))
+    eq, es = quantize64(x)
+    assert torch.equal(y.cpu(), (eq.double() @ w.double().t()).float() * es[:, None])
+
+
+def test_quantize_entry_pads_past_an_int_of_bits(device):
+    """Padding that begins 2^26 and more values behind the row: still 0."""
+    from ldsgnn import _native as nat
+    cols, ldq = 9, (1 << 26) + 4096
+    x = torch.arange(1.0, cols + 1.0, device=device)
+    q = torch.full((ldq,), 85, dtype=torch.int8, device=device)
+    scale = torch.empty(1, device=device)
+    nat.call("lds_quantize_rows", x.data_ptr(), cols, 1, cols, 0, q.data_ptr(), ldq, scale.data_ptr(),
+             nat.stream_of(x.device))
+    assert torch.equal(q[:cols].cpu(), quantize64(x.cpu()[None])[0][0]) and not q[cols:].any()
+
+
 def ints(g, *shape):
     return torch.randint(-127, 128, shape, generator=g, dtype=torch.int8)
 
