@@ -377,6 +377,70 @@ def test_group_norm_backward(device, ops, shape, dtype, act, p):
         assert err.max() <= 0, (name, float(err.max()))
 
 
+# Long rows whose vectors fill more than one block across (two or three chunks of
+# whole groups, the last one shorter): 37 groups of 64 in chunks of 19 and 18 (16-bit)
+# or 13, 13 and 11 (fp32); 101 of 12 in 51 and 50; 300 of 2 in two of 150.
+NORM_CHUNK_SHAPES = [(2, 601, 37, 64), (1, 3001, 101, 12), (4, 1501, 300, 2)]
+
+
+@pytest.mark.parametrize("shape", NORM_CHUNK_SHAPES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,p", [("silu", 0.1), ("none", 0.5)])
+def test_group_norm_in_chunks(device, ops, shape, dtype, act, p):
+    from ldsgnn import _native as nat
+    s, n, groups, cg = shape
+    code = nat.ELEMENT_CODES[dtype]
+    assert nat.lib.lds_group_norm_ws_bytes(s, n, groups * cg, groups, code, 0) > 0  # rows cut into parts
+    test_group_norm_forward(device, ops, shape, dtype, act, p)
+    test_group_norm_backward(device, ops, shape, dtype, act, p)
+
+
+def mask_columns(key, rows, cols, p):
+    """mask64 at some columns."""
+    quads = np.arange((rows + 3) // 4)[:, None]
+    words = philox.philox4x32_10(np.asarray(cols)[None, :], quads, key[1], key[2], key[0] & 0xFFFFFFFF, key[0] >> 32)
+    u = np.stack([(w >> np.uint64(8)).astype(np.float64) * 2.0 ** -24 for w in words], 1)
+    keep = np.float32(1.0) - np.float32(p)
+    return torch.from_numpy(u.reshape(-1, len(cols))[:rows] < keep), float(np.float32(1.0) / keep)
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 14001), (torch.float32, 7001)])
+def test_group_norm_results_past_the_caches(device, ops, dtype, n):
+    """147 MB results (y and dx are stored past the caches, x and dy read past
+    them) of 41 groups of 64 in two (bf16) or three chunks: forward, dx, dγ and dβ
+    of the groups at the chunks' borders against 64 bits, under the bounds of
+    test_group_norm_forward and _backward."""
+    s, groups, cg, p = 2, 41, 64, 0.2
+    c = groups * cg
+    g = torch.Generator(device=device).manual_seed(n)
+    x = torch.randn(s, n, c, generator=g, device=device).mul_(1.5).add_(0.3).to(dtype).requires_grad_()
+    dy = torch.randn(s, n, c, generator=g, device=device).to(dtype)
+    w = torch.randn(c, generator=g, device=device).mul_(0.3).add_(1.0).requires_grad_()
+    b = torch.randn(c, generator=g, device=device).mul_(0.3).requires_grad_()
+    assert x.numel() * x.element_size() > 128 << 20
+    y = ops.group_norm_act(x, groups, w, b, act="silu", p=p, key=KEY)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    y = y.detach()
+    pick = [0, 13, 14, 20, 21, 40]
+    cols = torch.cat([torch.arange(k * cg, (k + 1) * cg) for k in pick])
+    kept, scale = mask_columns(KEY, s * n, cols.numpy(), p)
+    kept = kept.to(device).view(s, n, -1)
+    cut = [t.detach()[..., cols.to(device)] for t in (x, w, b, dy)]
+    leaves = [t.double().requires_grad_() for t in cut[:3]]
+    a, z = norm64(leaves[0], len(pick), leaves[1], leaves[2], "silu", 1e-5, KEY, 0.0)
+    ref = torch.where(kept, a * scale, torch.zeros_like(a))
+    refs = torch.autograd.grad(ref, leaves, cut[3].double())
+    ref, z = ref.detach(), z.detach()
+    dz, _, _ = norm_bounds(leaves[0].detach(), len(pick), leaves[1].detach(), leaves[2].detach(), 1e-5)
+    tol = HALF[dtype] * ref.abs() + TINY[dtype] + 1.25 * (1.1 * dz + 8 * U * z.abs())
+    assert ((y[..., cols.to(device)].double() - ref).abs() <= tol).all()
+    tols = grad_bounds(cut[0], len(pick), cut[1], cut[2], "silu", p, cut[3])
+    for name, got, e, t, dt in zip(("dx", "dweight", "dbias"), (dx, dw, db), refs, tols,
+                                   (dtype, torch.float32, torch.float32)):
+        err = (got[..., cols.to(device)].double() - e).abs() - HALF[dt] * e.abs() - TINY[dt] - t
+        assert err.max() <= 0, (name, float(err.max()))
+
+
 def test_group_norm_gradient_by_differences(device, ops):
     """The gradient against central differences of the kernel's own forward
     (fp32): along a random direction d, (L(x + t d) - L(x - t d)) / 2t with t = 2^-6
@@ -647,6 +711,32 @@ def test_int8_matmul_whole_numbers(device, ops, m, n, k):
         y127 = ops.int8_linear(a127.float().to(device), b.to(device), one[:n])
     assert torch.equal(y127.cpu(), (a127.double() @ b.double().t()).float())
     assert torch.equal(y.cpu(), (a.double() @ b.double().t()).float())
+
+
+def int8_tile(m, n):
+    """The largest tile that gives 192 blocks (lds_int8_matmul's rule), 0: split."""
+    for bm, bn in ((256, 256), (256, 128), (128, 128), (128, 64), (64, 64)):
+        if -(-m // bm) * -(-n // bn) >= 192:
+            return bm, bn
+    return 0
+
+
+@pytest.mark.parametrize("m,n,k,tile", [
+    (3590, 3587, 1031, (256, 256)), (3585, 3841, 448, (256, 256)), (2500, 3300, 777, (256, 128)),
+    (2561, 3205, 1024, (256, 128)), (1600, 2000, 1000, (128, 128)), (1665, 1793, 833, (128, 128)),
+    (1500, 1090, 1033, (128, 64)), (1030, 810, 1409, (64, 64))])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_int8_tiles_in_their_steady_loop(device, ops, m, n, k, tile, dtype):
+    """Every tile instance over seven and more steps of 64 bytes, so that its ring
+    is refilled in the loop (from six steps on; eight with the longer ring), with
+    ends of m, n and k inside a tile, a step and a 16-byte chunk: whole numbers,
+    exact."""
+    assert int8_tile(m, n) == tile and (k + 63) // 64 >= 7
+    g = torch.Generator().manual_seed(m + n + k)
+    a, b = (ints(g, r, k).to(device) for r in (m, n))
+    one = torch.ones(max(m, n), device=device)
+    y = ops.int8_matmul(a, one[:m], b, one[:n], out_dtype=dtype)
+    assert torch.equal(y, (a.double() @ b.double().t()).float().to(dtype))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
