@@ -75,7 +75,7 @@ int launch_dropout(const T* x, int64_t ldx, const T* residual, int64_t ldr, T* y
     const int cvecs = (cols - 1) / V + 1;
     const int64_t total = (rows + 3) / 4 * cvecs;
     const int64_t blocks = (total + 255) / 256;
-    LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
+    LDS_CHECK_ARG(grid_fits(blocks, 256));
     const auto span = [&](const T* p, int64_t ld) { return ByteSpan(p, (rows - 1) * ld + cols, sizeof(T)); };
     const ByteSpan to = span(y, ldy);
     const bool whole = !to.meets(span(x, ldx)) && !(residual && to.meets(span(residual, ldr)));

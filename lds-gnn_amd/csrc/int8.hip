@@ -641,7 +641,7 @@ namespace {
 template <typename T, int MF, int NF, int W>
 int launch_split(const Int8Args& a, T* y, hipStream_t st) {
     const int64_t blocks = ((a.m + 16 * MF - 1) / (16 * MF)) * ((a.n + 16 * NF - 1) / (16 * NF));
-    LDS_CHECK_ARG(blocks < (int64_t)1 << 31);
+    LDS_CHECK_ARG(grid_fits(blocks, 64 * W));
     hipLaunchKernelGGL((int8_split_kernel<T, MF, NF, W>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a, y);
     LDS_RETURN_LAST_ERROR();
 }
@@ -649,7 +649,7 @@ int launch_split(const Int8Args& a, T* y, hipStream_t st) {
 template <typename T, int BM, int BN, int WM, int WN, int S>
 int launch_tile(const Int8Args& a, T* y, hipStream_t st) {
     const int64_t tiles = ((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN);
-    LDS_CHECK_ARG(tiles < (int64_t)1 << 30);
+    LDS_CHECK_ARG(tiles < (int64_t)1 << 30 && grid_fits(tiles + 7, 64 * WM * WN));
     const unsigned blocks = (unsigned)((tiles + 7) / 8 * 8);  // whole rounds of the eight XCDs
     hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WM, WN, S>), dim3(blocks), dim3(64 * WM * WN), 0, st, a, y);
     LDS_RETURN_LAST_ERROR();
@@ -667,9 +667,12 @@ extern "C" int lds_quantize_rows(const void* x, int64_t ldx, int64_t rows, int c
         using T = decltype(zero);
         constexpr int V = 16 / (int)sizeof(T);
         auto go = [&](auto lanes, auto regs) {
-            constexpr int G = decltype(lanes)::value, R = decltype(regs)::value;
-            hipLaunchKernelGGL((quantize_rows_kernel<T, V, G, R>), dim3((unsigned)((rows + 256 / G - 1) / (256 / G))),
-                               dim3(256), 0, (hipStream_t)stream, (const T*)x, ldx, rows, cols, q, ldq, scale);
+            constexpr int G = decltype(lanes)::value, R = decltype(regs)::value, kRows = 256 / G;
+            in_launches((rows + kRows - 1) / kRows, 256, [&](int64_t first, unsigned blocks) {
+                const int64_t r = first * kRows;
+                hipLaunchKernelGGL((quantize_rows_kernel<T, V, G, R>), dim3(blocks), dim3(256), 0, (hipStream_t)stream,
+                                   (const T*)x + r * ldx, ldx, rows - r, cols, q + r * ldq, ldq, scale + r);
+            });
         };
         // a row in the registers of 16 or 32 lanes, of a wave or of a block
         if (ldq <= 16 * V)
@@ -727,13 +730,13 @@ extern "C" int lds_int8_linear(const void* x, int64_t ldx, int xdtype, signed ch
     LDS_CHECK_ARG(xs && ws && y && ldy >= n);
     LDS_CHECK_ARG(k == 0 || (q && wq && ldq >= k && ldw >= k && ldq % 16 == 0 && ldw % 16 == 0 &&
                              (((uintptr_t)q | (uintptr_t)wq) & 15) == 0));
-    if (k > 0 && m <= kFewRows && m * ldq <= kFewBytes) {
+    if (k > 0 && m <= kFewRows && m * ldq <= kFewBytes && grid_fits(((int64_t)n + 15) / 16, 512)) {
         LDS_CHECK_ARG(x && ldx >= k && xdtype >= LDS_F32 && xdtype <= LDS_F16);
         return with_type(xdtype, [&](auto zero) -> int {
             using TX = decltype(zero);
             constexpr int V = 16 / (int)sizeof(TX);
             const Int8Args a{nullptr, wq, nullptr, ws, bias, 0, ldw, ldy, m, n, k, ptype};
-            hipLaunchKernelGGL((int8_few_kernel<TX, V>), dim3((unsigned)((n + 15) / 16)), dim3(512), 0,
+            hipLaunchKernelGGL((int8_few_kernel<TX, V>), dim3((unsigned)(((int64_t)n + 15) / 16)), dim3(512), 0,
                                (hipStream_t)stream, (const TX*)x, ldx, a, (int)ldq, y, dtype);
             LDS_RETURN_LAST_ERROR();
         });

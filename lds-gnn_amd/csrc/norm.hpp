@@ -38,6 +38,7 @@ struct NormArgs {
     int whole;        // ... and a row's last one is stored whole (whole_store)
     int parts;        // row parts per sample
     int64_t part_q;   // row quads per part
+    unsigned first;   // blocks of the launches before this one
     const void* weight;
     const void* bias;
     int ptype;
@@ -91,7 +92,7 @@ __device__ __forceinline__ NormPlace norm_place(const NormArgs& a, int v, int64_
 }
 
 __device__ __forceinline__ NormPlace norm_part_place(const NormArgs& a, int v) {
-    const unsigned b = blockIdx.x, row = b / (unsigned)a.chunks;
+    const unsigned b = blockIdx.x + a.first, row = b / (unsigned)a.chunks;
     const unsigned s = row / (unsigned)a.parts;
     return norm_place(a, v, s, (int)(row - s * a.parts), (int)(b - row * a.chunks));
 }
@@ -477,6 +478,15 @@ inline int64_t backward_ws(const NormArgs& a, bool slab) {
     return a.samples * a.parts * (int64_t)a.c * 8 + a.samples * a.groups * 8;
 }
 
+// f(arguments, blocks) for the launches of a pass.
+template <typename F>
+inline void norm_launches(NormArgs a, int64_t blocks, int threads, F&& f) {
+    in_launches(blocks, threads, [&](int64_t first, unsigned count) {
+        a.first = (unsigned)first;
+        f(a, count);
+    });
+}
+
 // Blocks of a slab launch, and a block's place in it: the blocks of a sample
 // share its lines where a group is narrow, so from eight samples on a sample
 // stays on one XCD (blocks go round the eight of them).
@@ -484,7 +494,7 @@ inline int64_t slab_blocks(const NormArgs& a) {
     return a.samples >= 8 ? (a.samples + 7) / 8 * 8 * a.chunks : a.samples * a.chunks;
 }
 __device__ __forceinline__ bool slab_place(const NormArgs& a, int64_t& s, int& chunk) {
-    const unsigned b = blockIdx.x, u = a.samples >= 8 ? b >> 3 : b;
+    const unsigned b = blockIdx.x + a.first, u = a.samples >= 8 ? b >> 3 : b;
     const unsigned t = u / (unsigned)a.chunks;
     chunk = (int)(u - t * a.chunks);
     s = a.samples >= 8 ? (int64_t)t * 8 + (b & 7) : t;

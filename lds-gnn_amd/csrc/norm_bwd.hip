@@ -267,10 +267,11 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
                                                                       float* __restrict__ dbias) {
     __shared__ double red[2][kNormThreads];
     const int t = threadIdx.x;
+    const unsigned b = blockIdx.x + a.first;
     double h = 0.0, hx = 0.0;
-    if ((int64_t)blockIdx.x < pairs) {
-        const int64_t s = blockIdx.x / a.groups;
-        const int g = (int)(blockIdx.x - s * a.groups);
+    if ((int64_t)b < pairs) {
+        const int64_t s = b / (unsigned)a.groups;
+        const int g = (int)(b - s * a.groups);
         const int64_t items = (int64_t)a.parts * a.cg;
 #pragma unroll 4
         for (int64_t i = t; i < items; i += kNormThreads) {
@@ -290,12 +291,12 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
         __syncthreads();
         if (t == 0) {
             const double m = (double)a.n * (double)a.cg;
-            means[blockIdx.x] = make_float2((float)((red[0][0] + red[0][1] + red[0][2] + red[0][3]) / m),
+            means[b] = make_float2((float)((red[0][0] + red[0][1] + red[0][2] + red[0][3]) / m),
                                             (float)((red[1][0] + red[1][1] + red[1][2] + red[1][3]) / m));
         }
         return;
     }
-    const int c = (int)(blockIdx.x - pairs) * 4 + (t & 3);
+    const int c = (int)(b - pairs) * 4 + (t & 3);
     const int64_t rows = a.samples * a.parts;
     if (c < a.c) {
 #pragma unroll 4
@@ -416,24 +417,32 @@ extern "C" int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy
                     constexpr bool DROP = decltype(dr)::value;
                     auto slab = [&](auto qc) {
                         const bool direct = samples == 1;
-                        hipLaunchKernelGGL((gn_bwd_slab_kernel<T, V, ACT, DROP, decltype(qc)::value>),
-                                           dim3((unsigned)blocks), dim3(k.threads), 0, st, (const T*)dy, sdy, lddy,
-                                           (const T*)x, a, mean, rstd, params && !direct ? sums : nullptr,
-                                           direct ? dweight : nullptr, direct ? dbias : nullptr, (T*)dx);
+                        norm_launches(a, blocks, k.threads, [&](const NormArgs& l, unsigned count) {
+                            hipLaunchKernelGGL((gn_bwd_slab_kernel<T, V, ACT, DROP, decltype(qc)::value>), dim3(count),
+                                               dim3(k.threads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, l, mean,
+                                               rstd, params && !direct ? sums : nullptr, direct ? dweight : nullptr,
+                                               direct ? dbias : nullptr, (T*)dx);
+                        });
                     };
                     if (!k.slab)
-                        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP, SPAN>), dim3((unsigned)blocks),
-                                           dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, a, mean,
-                                           rstd, sums);
+                        norm_launches(a, blocks, kNormThreads, [&](const NormArgs& l, unsigned count) {
+                            hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, ACT, DROP, SPAN>), dim3(count),
+                                               dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, l, mean,
+                                               rstd, sums);
+                        });
                     else if constexpr (!SPAN)
                         with_quads<V>(k.quads, slab);
-                    if (cblocks)
-                        hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3((unsigned)cblocks), dim3(kNormThreads), 0, st,
-                                           (const float2*)sums, a, pairs, means, dweight, dbias);
+                    norm_launches(a, cblocks, kNormThreads, [&](const NormArgs& l, unsigned count) {
+                        hipLaunchKernelGGL(gn_bwd_combine_kernel, dim3(count), dim3(kNormThreads), 0, st,
+                                           (const float2*)sums, l, pairs, means, dweight, dbias);
+                    });
                     auto second = [&](auto ps) {
-                        hipLaunchKernelGGL((gn_bwd_dx_kernel<T, V, ACT, DROP, SPAN, WIDE ? decltype(ps)::value : 0>),
-                                           dim3((unsigned)blocks), dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy,
-                                           (const T*)x, a, mean, rstd, (const float2*)means, (T*)dx);
+                        norm_launches(a, blocks, kNormThreads, [&](const NormArgs& l, unsigned count) {
+                            hipLaunchKernelGGL(
+                                (gn_bwd_dx_kernel<T, V, ACT, DROP, SPAN, WIDE ? decltype(ps)::value : 0>),
+                                dim3(count), dim3(kNormThreads), 0, st, (const T*)dy, sdy, lddy, (const T*)x, l, mean,
+                                rstd, (const float2*)means, (T*)dx);
+                        });
                     };
                     if (!k.slab && dx) past == 2 ? second(IntC<2>{}) : past ? second(IntC<1>{}) : second(IntC<0>{});
                 };

@@ -381,28 +381,37 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
             constexpr int V = decltype(vc)::value;
             constexpr bool SPAN = decltype(sc)::value, WIDE = !SPAN && V * sizeof(T) == 16;
             if (!k.slab) {
-                if constexpr (SPAN)
-                    hipLaunchKernelGGL((gn_stats_span_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0,
-                                       st, (const T*)x, a, (Moments*)ws);
-                else
-                    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3((unsigned)blocks), dim3(kNormThreads), 0, st,
-                                       (const T*)x, a, (Moments*)ws);
-                hipLaunchKernelGGL(gn_combine_kernel, dim3((unsigned)((pairs + 3) / 4)), dim3(kNormThreads), 0, st,
-                                   (const Moments*)ws, pairs, a.parts * a.sub, eps, mean, rstd);
+                norm_launches(a, blocks, kNormThreads, [&](const NormArgs& l, unsigned count) {
+                    if constexpr (SPAN)
+                        hipLaunchKernelGGL((gn_stats_span_kernel<T, V>), dim3(count), dim3(kNormThreads), 0, st,
+                                           (const T*)x, l, (Moments*)ws);
+                    else
+                        hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3(count), dim3(kNormThreads), 0, st,
+                                           (const T*)x, l, (Moments*)ws);
+                });
+                in_launches((pairs + 3) / 4, kNormThreads, [&](int64_t first, unsigned count) {
+                    const int64_t i = first * 4, each = (int64_t)a.parts * a.sub;
+                    hipLaunchKernelGGL(gn_combine_kernel, dim3(count), dim3(kNormThreads), 0, st,
+                                       (const Moments*)ws + i * each, pairs - i, (int)each, eps, mean + i, rstd + i);
+                });
             }
             return with_act(act, [&](auto ac) -> int {
                 constexpr int ACT = decltype(ac)::value;
                 auto go = [&](auto dr) {
                     constexpr bool DROP = decltype(dr)::value;
                     auto slab = [&](auto qc) {
-                        hipLaunchKernelGGL((gn_slab_kernel<T, V, ACT, DROP, decltype(qc)::value>),
-                                           dim3((unsigned)blocks), dim3(k.threads), 0, st, (const T*)x, a, eps, (T*)y,
-                                           mean, rstd);
+                        norm_launches(a, blocks, k.threads, [&](const NormArgs& l, unsigned count) {
+                            hipLaunchKernelGGL((gn_slab_kernel<T, V, ACT, DROP, decltype(qc)::value>), dim3(count),
+                                               dim3(k.threads), 0, st, (const T*)x, l, eps, (T*)y, mean, rstd);
+                        });
                     };
                     auto apply = [&](auto ps) {
-                        hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP, SPAN, WIDE && decltype(ps)::value>),
-                                           dim3((unsigned)(samples * b.parts * b.chunks)), dim3(kNormThreads), 0, st,
-                                           (const T*)x, b, mean, rstd, (T*)y);
+                        norm_launches(b, samples * b.parts * b.chunks, kNormThreads,
+                                      [&](const NormArgs& l, unsigned count) {
+                            hipLaunchKernelGGL((gn_apply_kernel<T, V, ACT, DROP, SPAN, WIDE && decltype(ps)::value>),
+                                               dim3(count), dim3(kNormThreads), 0, st, (const T*)x, l, mean, rstd,
+                                               (T*)y);
+                        });
                     };
                     if (!k.slab)
                         past ? apply(BoolC<true>{}) : apply(BoolC<false>{});

@@ -230,6 +230,18 @@ inline bool drop_key(float keep, float scale, uint64_t seed, uint32_t tag, uint3
     return t < 16777216.0;
 }
 
+// A launch counts its threads along x in 32 bits, and one with more runs in part,
+// with no error: no launch has more.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= 0xffffffffll / threads; }
+// f(first block, blocks) for the launches that `blocks` of them take: whole
+// rounds of the eight XCDs each.
+template <typename F>
+inline void in_launches(int64_t blocks, int threads, F&& f) {
+    const int64_t most = 0xffffffffll / threads / 8 * 8;
+    for (int64_t first = 0; first < blocks; first += most)
+        f(first, (unsigned)(blocks - first < most ? blocks - first : most));
+}
+
 // A compile-time int as a value.
 template <int N>
 struct IntC {

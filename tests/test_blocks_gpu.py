@@ -233,6 +233,58 @@ def test_offsets_past_32_bits(device, ops):
     assert torch.equal(p[-300:], ref.float().to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("samples,groups,cg,dtype", [(70_000_001, 1, 8, torch.bfloat16),
+                                                     (25_000_003, 3, 2, torch.float16)])
+def test_group_norm_of_more_samples_than_a_launch_holds(device, ops, samples, groups, cg, dtype):
+    """Single nodes as samples, whose blocks have more than 2^32 threads, with a
+    sample's groups in one block and across blocks: y and dx, from the first
+    sample to the last, against 64 bits."""
+    c = groups * cg
+    g = torch.Generator(device=device).manual_seed(5)
+    x = torch.randn(samples, 1, c, generator=g, device=device, dtype=dtype)
+    dy = torch.randn(samples, 1, c, generator=g, device=device, dtype=dtype)
+    pl = ops._NormPlan(groups, ops.ACTIVATIONS["silu"], 1e-5, 1.0, 1.0, None)
+    y, stats = ops._norm_forward(x, None, None, pl)
+    dx = ops._norm_backward(dy, x, None, None, stats, pl, (True, False, False))[0]
+    pick = torch.cat([torch.randint(0, samples, (5000,), generator=g, device=device),
+                      torch.arange(samples - 100, samples, device=device), torch.arange(100, device=device)])
+    xs, ds = x[pick].cpu(), dy[pick].cpu()
+    one, zero = torch.ones(c).double(), torch.zeros(c).double()
+    ref, z = norm64(xs.double(), groups, None, None, "silu", 1e-5, KEY, 0.0)
+    dz, _, _ = norm_bounds(xs.double(), groups, None, None, 1e-5)
+    tol = HALF[dtype] * ref.abs() + TINY[dtype] + 1.1 * dz + 8 * U * z.abs()
+    assert ((y[pick].cpu().double() - ref).abs() <= tol).all()
+    rx = norm_grads64(xs, groups, one, zero, "silu", 0.0, ds)[0][0]
+    tx = grad_bounds(xs, groups, one, zero, "silu", 0.0, ds)[0]
+    assert ((dx[pick].cpu().double() - rx).abs() <= HALF[dtype] * rx.abs() + TINY[dtype] + tx).all()
+
+
+def test_quantize_more_rows_than_a_launch_holds(device, ops):
+    """300 million rows of one value: q = 127 times its sign, scale = |x| / 127 (in 64
+    bits, then rounded: torch divides an fp32 tensor by a number as a product with
+    the number's rounded reciprocal.  A quotient by 127 is 2^-32 or more of itself
+    away from the middle of two fp32 values, 64 bits err by 2^-52.)"""
+    x = torch.rand(300_000_001, 1, device=device).sub_(0.5)
+    q, s = ops.quantize_rows(x)
+    for i in range(0, x.size(0), 50_000_000):
+        v = x[i:i + 50_000_000, 0]
+        assert torch.equal(q[i:i + 50_000_000, 0].float(), v.sign() * 127)
+        assert torch.equal(s[i:i + 50_000_000], (v.abs().double() / 127).float())
+
+
+def test_int8_linear_of_more_columns_than_a_launch_holds(device, ops):
+    """One row times 135 million rows of w: the one-launch form would need more
+    than 2^32 threads."""
+    n, k = 135_000_003, 16
+    wq = torch.randint(-127, 128, (n, k), dtype=torch.int8, device=device)
+    x = torch.arange(k, device=device).float().sub_(8)[None]
+    x[0, 3] = 127
+    with torch.no_grad():
+        y = ops.int8_linear(x, wq, torch.ones(1, device=device).expand(n))
+    for i in range(0, n, 20_000_000):
+        assert torch.equal(y[0, i:i + 20_000_000], (wq[i:i + 20_000_000].float() * x).sum(1))
+
+
 # ---------------------------------------------------------------------------
 # group norm + activation
 # ---------------------------------------------------------------------------
