@@ -479,7 +479,9 @@ int lds_dropout(const float* x, int ldx, float* y, int ldy, int rows, int cols,
  * same call on dy, without a residual, is the backward.  Rows may start at any
  * element (row strides ldx, ldr, ldy in elements; no alignment is needed).
  * keep_prob in [0, 1]; a dropped element is 0 (+ residual) whatever x holds
- * there.  y does not overlap x or residual. */
+ * there.  y may be x or residual itself (the same address and row stride), or
+ * other columns of the same rows; it overlaps neither in any other way.  The
+ * same holds for lds_dropout. */
 int lds_dropout_add(const void* x, int64_t ldx, const void* residual,
                     int64_t ldr, void* y, int64_t ldy, int64_t rows, int cols,
                     int dtype, float keep_prob, float scale, uint64_t seed,
@@ -498,6 +500,8 @@ int lds_dropout_add(const void* x, int64_t ldx, const void* residual,
  * samples × groups fp32, kept for the backward.  ws: lds_group_norm_ws_bytes
  * bytes, 16-byte aligned, any contents, not shared by calls that may run at
  * the same time.
+ * y may be x itself, where x is contiguous; it does not overlap x in any other
+ * way, nor anything else.
  * Statistics are fp32 sums about an element of their own group, combined as
  * (count, mean, centred sum of squares); the last combination is fp64.
  * ------------------------------------------------------------------------- */
@@ -517,6 +521,8 @@ int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx,
  * and the key);  dweight_c = Σ h x̂,  dbias_c = Σ h  (fp32, c each; NULL: not
  * wanted),  dx = rstd (γ h - mean_g(γ h) - x̂ mean_g(γ h x̂))  (contiguous; NULL:
  * not wanted).  relu'(0) = 0.  dy: strides sdy, lddy, channels contiguous.
+ * dx may be dy or x itself, where that is contiguous; otherwise outputs and
+ * inputs do not overlap.
  * Sums run in a fixed order: equal calls give equal bits. */
 int lds_group_norm_backward(const void* dy, int64_t sdy, int64_t lddy,
                             const void* x, int64_t sx, int64_t ldx,

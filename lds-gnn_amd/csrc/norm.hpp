@@ -35,7 +35,7 @@ struct NormArgs {
     int chunks;       // blocks across a row
     int lpg, sub;     // vectors per group (in the chunk); chunks per group
     int span;         // vectors lie across groups (norm_plan says when)
-    int whole;        // ... and a row's last one is stored whole (whole_store)
+    int whole;        // the result overlaps no input; across groups a row's last vector is stored whole (whole_store)
     int parts;        // row parts per sample
     int64_t part_q;   // row quads per part
     unsigned first;   // blocks of the launches before this one
@@ -115,7 +115,7 @@ struct Quad {
     Raw<T, V> row[4];
 
     template <bool PAST = false>
-    __device__ __forceinline__ void load(const T* __restrict__ base, int64_t ld, const NormPlace& p, int64_t q,
+    __device__ __forceinline__ void load(const T* base, int64_t ld, const NormPlace& p, int64_t q,
                                          const QuadRows& in) {
         const T* at = base + (4 * q - p.f0) * ld;
 #pragma unroll
@@ -298,7 +298,7 @@ struct NormParams {
 
 // A thread's vector of a row; at a row's end across groups only what it owns.
 template <typename T, int V, bool SPAN, bool PAST = false>
-__device__ __forceinline__ void store_own(T* __restrict__ at, int skip, const float (&o)[V]) {
+__device__ __forceinline__ void store_own(T* at, int skip, const float (&o)[V]) {
     if constexpr (SPAN) {
         if (skip) {
 #pragma unroll

@@ -45,7 +45,7 @@ struct BackQuad {
     // dx = (γ rstd scale) h + (-(rstd² m2) (x - mean) - rstd m1)
     template <bool PAST>
     __device__ __forceinline__ void store(const QuadRows& in, const float (&rws)[V], const GroupValue<V, SPAN>& k0,
-                                          const GroupValue<V, SPAN>& k1, T* __restrict__ at, int64_t ld,
+                                          const GroupValue<V, SPAN>& k1, T* at, int64_t ld,
                                           int skip) const {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -117,9 +117,9 @@ __device__ __forceinline__ int chunk_last(const NormArgs& a, int chunk) {
 
 template <typename T, int V, int ACT, bool DROP, int Q>
 __global__ __launch_bounds__(kBackwardSlabThreads) void gn_bwd_slab_kernel(
-    const T* __restrict__ dy, int64_t sdy, int64_t lddy, const T* __restrict__ x, NormArgs a,
-    const float* __restrict__ mean, const float* __restrict__ rstd, float2* __restrict__ sums,
-    float* __restrict__ dweight, float* __restrict__ dbias, T* __restrict__ dx) {
+    const T* dy, int64_t sdy, int64_t lddy, const T* x, NormArgs a, const float* __restrict__ mean,
+    const float* __restrict__ rstd, float2* __restrict__ sums, float* __restrict__ dweight, float* __restrict__ dbias,
+    T* dx) {
     constexpr int NT = kBackwardSlabThreads;
     __shared__ float2 chan[V][NT];
     __shared__ float2 red[2 * NT];
@@ -323,12 +323,11 @@ __global__ __launch_bounds__(kNormThreads) void gn_bwd_combine_kernel(const floa
 
 // PAST: x and dy are read past the caches (1), dx is stored past them too (2).
 template <typename T, int V, int ACT, bool DROP, bool SPAN, int PAST>
-__global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* __restrict__ dy, int64_t sdy, int64_t lddy,
-                                                                 const T* __restrict__ x, NormArgs a,
+__global__ __launch_bounds__(kNormThreads) void gn_bwd_dx_kernel(const T* dy, int64_t sdy, int64_t lddy, const T* x,
+                                                                 NormArgs a,
                                                                  const float* __restrict__ mean,
                                                                  const float* __restrict__ rstd,
-                                                                 const float2* __restrict__ means,
-                                                                 T* __restrict__ dx) {
+                                                                 const float2* __restrict__ means, T* dx) {
     const NormPlace p = norm_part_place(a, V);
     if (!p.live) return;
     GroupValue<V, SPAN> mu, rs, k0, k1;

@@ -13,7 +13,7 @@ struct Moments {
 template <typename T, int V, int ACT, bool DROP, bool SPAN, bool PAST = false>
 __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& in, const NormParams<V>& par,
                                            const GroupValue<V, SPAN>& mu, const bool (&kept)[4][V], float scale,
-                                           T* __restrict__ at, int64_t ld, int skip) {
+                                           T* at, int64_t ld, int skip) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         if (r < in.lo || r >= in.hi) continue;
@@ -35,9 +35,8 @@ __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& 
 // ---------------------------------------------------------------------------
 
 template <typename T, int V, int ACT, bool DROP, int Q>
-__global__ __launch_bounds__(1024) void gn_slab_kernel(const T* __restrict__ x, NormArgs a, float eps,
-                                                       T* __restrict__ y, float* __restrict__ mean,
-                                                       float* __restrict__ rstd) {
+__global__ __launch_bounds__(1024) void gn_slab_kernel(const T* x, NormArgs a, float eps, T* y,
+                                                       float* __restrict__ mean, float* __restrict__ rstd) {
     __shared__ float2 red[2][2 * 1024];
     int64_t s;
     int chunk;
@@ -304,11 +303,12 @@ __global__ __launch_bounds__(kNormThreads) void gn_combine_kernel(const Moments*
     }
 }
 
-// PAST: x is read and y stored past the caches.
+// PAST: x is read and y stored past the caches, and they do not overlap (16 x 20000 x
+// 256 fp32 with dropout 109 us; 122 where the compiler cannot know it).
 template <typename T, int V, int ACT, bool DROP, bool SPAN, bool PAST>
-__global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(const T* __restrict__ x, NormArgs a,
+__global__ __launch_bounds__(kNormThreads) void gn_apply_kernel(Pointer<const T, PAST> x, NormArgs a,
                                                                 const float* __restrict__ mean,
-                                                                const float* __restrict__ rstd, T* __restrict__ y) {
+                                                                const float* __restrict__ rstd, Pointer<T, PAST> y) {
     const NormPlace p = norm_part_place(a, V);
     if (!p.live) return;
     GroupValue<V, SPAN> mu, rs;
@@ -373,7 +373,7 @@ extern "C" int lds_group_norm_forward(const void* x, int64_t sx, int64_t ldx, in
     const int64_t pairs = samples * groups;
     LDS_CHECK_ARG(blocks < (int64_t)1 << 31 && samples * b.parts * b.chunks < (int64_t)1 << 31);
     LDS_CHECK_ARG(pairs < (int64_t)1 << 32);
-    const bool past = past_caches(samples * n * c * size) && whole_lines(x, samples, sx, ldx, c, size) &&
+    const bool past = a.whole && past_caches(samples * n * c * size) && whole_lines(x, samples, sx, ldx, c, size) &&
                       whole_lines(y, 1, 0, c, c, size);
     return with_type(dtype, [&](auto zero) -> int {
         using T = decltype(zero);

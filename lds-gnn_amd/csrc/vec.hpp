@@ -6,6 +6,8 @@
 // even, when it is stored.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "../../include/ldsgnn.h"
 
@@ -25,6 +27,9 @@ struct ByteSpan {
     bool meets(const ByteSpan& o) const { return lo < o.hi && o.lo < hi; }
 };
 
+// The helpers' pointers are not __restrict__: a caller may write its result over an
+// input (include/ldsgnn.h says which).
+//
 // V consecutive elements as one load or store.  Rows of an odd length start at
 // any multiple of the element size: the type carries the element's alignment,
 // and gfx950's global memory takes a 16-byte access at any address.
@@ -38,7 +43,7 @@ struct VecOf<T, 1> {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[V]) {
+__device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) {
     if constexpr (V == 1) {
         f[0] = (float)p[0];
     } else {
@@ -50,7 +55,7 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[V])
 
 // PAST: a store that leaves the caches to others.
 template <typename T, int V, bool PAST = false>
-__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V]) {
+__device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
     if constexpr (V == 1) {
         p[0] = (T)f[0];
     } else {
@@ -66,7 +71,7 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[V]
 
 // A vector whose first w <= V elements exist (a row's last, partial one).
 template <typename T, int V>
-__device__ __forceinline__ void load_part(const T* __restrict__ p, int w, float (&f)[V]) {
+__device__ __forceinline__ void load_part(const T* p, int w, float (&f)[V]) {
     if (w >= V) {
         load_vec<T, V>(p, f);
         return;
@@ -75,7 +80,7 @@ __device__ __forceinline__ void load_part(const T* __restrict__ p, int w, float 
     for (int e = 0; e < V; ++e) f[e] = e < w ? (float)p[e] : 0.f;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_part(T* __restrict__ p, int w, const float (&f)[V]) {
+__device__ __forceinline__ void store_part(T* p, int w, const float (&f)[V]) {
     if (w >= V) {
         store_vec<T, V>(p, f);
         return;
@@ -97,7 +102,7 @@ template <typename T, int V>
 using Raw = typename VecOf<T, V>::type;
 // PAST: a last read, which leaves the caches to others.
 template <typename T, int V, bool PAST = false>
-__device__ __forceinline__ Raw<T, V> load_raw(const T* __restrict__ p) {
+__device__ __forceinline__ Raw<T, V> load_raw(const T* p) {
     if constexpr (PAST)
         return __builtin_nontemporal_load(reinterpret_cast<const Raw<T, V>*>(p));
     else
@@ -241,6 +246,10 @@ inline void in_launches(int64_t blocks, int threads, F&& f) {
     for (int64_t first = 0; first < blocks; first += most)
         f(first, (unsigned)(blocks - first < most ? blocks - first : most));
 }
+
+// A pointer that no other argument's memory overlaps (RESTRICT), or that one may.
+template <typename T, bool RESTRICT>
+using Pointer = std::conditional_t<RESTRICT, T* __restrict__, T*>;
 
 // A compile-time int as a value.
 template <int N>

@@ -947,6 +947,82 @@ def test_group_norm_entries_in_place(device, n, groups, cg):
     assert torch.equal(forward(here, here), y)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 1), (7, 3), (1031, 33), (520, 8), (301, 257)])
+def test_dropout_add_in_place(device, dtype, rows, cols):
+    """y over x, y over the residual, and all three the same: the bits of separate
+    tensors."""
+    from ldsgnn import _native as nat
+    g = torch.Generator().manual_seed(rows + cols)
+    x, r = (torch.randn(rows, cols, generator=g).to(dtype) for _ in range(2))
+    code = nat.ELEMENT_CODES[dtype]
+
+    def call(a, b, y):
+        nat.call("lds_dropout_add", a.data_ptr(), cols, 0 if b is None else b.data_ptr(), cols, y.data_ptr(), cols, rows,
+                 cols, code, 0.75, float(np.float32(1.0) / np.float32(0.75)), *KEY, nat.stream_of(y.device))
+        return y.cpu()
+
+    a, b = x.to(device), r.to(device)
+    want = plain_dropout(x, KEY, 0.25, r)
+    assert torch.equal(call(a, b, a), want)
+    a = x.to(device)
+    assert torch.equal(call(a, b, b), want) and torch.equal(a.cpu(), x)
+    a = x.to(device)
+    assert torch.equal(call(a, a, a), plain_dropout(x, KEY, 0.25, x))
+    a = x.to(device)
+    assert torch.equal(call(a, None, a), plain_dropout(x, KEY, 0.25))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("s,n,groups,cg", [(3, 2, 2, 8), (9, 60, 5, 3), (2, 601, 37, 64), (3, 5001, 5, 3), (1, 40, 1, 8200),
+                                           (1, 9001, 2, 4)])
+def test_group_norm_in_place_in_every_form(device, ops, dtype, s, n, groups, cg):
+    """y over x, dx over dy and dx over x, in one launch and in parts, a group per
+    vector, vectors across groups and groups across blocks."""
+    from ldsgnn import _native as nat
+    c, code = groups * cg, nat.ELEMENT_CODES[dtype]
+    x, w, b, dy = (t.to(device) for t in norm_inputs(s, n, groups, cg, dtype, seed=21))
+    pl = ops._NormPlan(groups, ops.ACTIVATIONS["silu"], 1e-5, 0.75, 4.0 / 3.0, KEY)
+    y, stats = ops._norm_forward(x, w, b, pl)
+    dx, dw, db = ops._norm_backward(dy, x, w, b, stats, pl, (True, True, True))
+    ws = torch.empty(max(nat.lib.lds_group_norm_ws_bytes(s, n, c, groups, code, k) for k in (0, 1)) + 16,
+                     dtype=torch.uint8, device=device)
+    st, at, to = nat.stream_of(x.device), stats.data_ptr(), stats.data_ptr() + 4 * s * groups
+    for over in ("dy", "x"):
+        a, d = x.clone(), dy.clone()
+        out = d if over == "dy" else a
+        ew, eb = torch.empty(c, device=device), torch.empty(c, device=device)
+        nat.call("lds_group_norm_backward", d.data_ptr(), n * c, c, a.data_ptr(), n * c, c, s, n, c, groups, code,
+                 w.data_ptr(), b.data_ptr(), 0, pl.act, *pl.mask, at, to, out.data_ptr(), ew.data_ptr(), eb.data_ptr(),
+                 ws.data_ptr(), st)
+        assert torch.equal(out, dx) and torch.equal(ew, dw) and torch.equal(eb, db), over
+    nat.call("lds_group_norm_forward", x.data_ptr(), n * c, c, s, n, c, groups, code, w.data_ptr(), b.data_ptr(), 0, 1e-5,
+             pl.act, *pl.mask, x.data_ptr(), at, to, ws.data_ptr(), st)
+    assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 14001), (torch.float32, 7001)])
+def test_group_norm_in_place_past_the_caches(device, ops, dtype, n):
+    """147 MB over itself: the bits of a result of its own, which is stored past
+    the caches."""
+    from ldsgnn import _native as nat
+    s, groups, c = 2, 41, 41 * 64
+    code = nat.ELEMENT_CODES[dtype]
+    x, dy = (torch.randn(s, n, c, device=device, dtype=dtype) for _ in range(2))
+    pl = ops._NormPlan(groups, ops.ACTIVATIONS["silu"], 1e-5, 0.75, 4.0 / 3.0, KEY)
+    y, stats = ops._norm_forward(x, None, None, pl)
+    dx = ops._norm_backward(dy, x, None, None, stats, pl, (True, False, False))[0]
+    ws = torch.empty(max(nat.lib.lds_group_norm_ws_bytes(s, n, c, groups, code, k) for k in (0, 1)), dtype=torch.uint8,
+                     device=device)
+    st, at, to = nat.stream_of(x.device), stats.data_ptr(), stats.data_ptr() + 4 * s * groups
+    nat.call("lds_group_norm_backward", dy.data_ptr(), n * c, c, x.data_ptr(), n * c, c, s, n, c, groups, code, 0, 0, 0,
+             pl.act, *pl.mask, at, to, dy.data_ptr(), 0, 0, ws.data_ptr(), st)
+    assert torch.equal(dy, dx)
+    nat.call("lds_group_norm_forward", x.data_ptr(), n * c, c, s, n, c, groups, code, 0, 0, 0, 1e-5, pl.act, *pl.mask,
+             x.data_ptr(), at, to, ws.data_ptr(), st)
+    assert torch.equal(x, y)
+
+
 def test_captured_run_replays_the_eager_bits(device, ops):
     """Forward, backward and the 8-bit product in one captured graph, replayed
     with new inputs and eager work in between; kernel nodes only."""
