@@ -23,7 +23,7 @@ from typing import List, Optional, Tuple
 
 import numpy as np
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from . import _native as nat
 from .rng import TAG_DROP_H, TAG_DROP_X, Generator, default_generator
@@ -45,6 +45,15 @@ def _f32c(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.size(1):
         return t
     return t.contiguous()
+
+
+def _no_tangent(what: str, *tensors) -> None:
+    """Forward-mode derivatives are not implemented: a tangent is refused, where
+    the direct launch would drop it."""
+    if forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"ldsgnn {what}: no forward-mode derivative; use reverse mode")
 
 
 # ---------------------------------------------------------------------------
@@ -392,6 +401,7 @@ class _Aggregate(Function):
 
 def aggregate(z: torch.Tensor, graph: CsrGraph) -> torch.Tensor:
     """Â·Z for a hot-path graph, differentiable in Z and (sampled graphs) θ."""
+    _no_tangent("aggregate", z)
     if isinstance(graph, SampledGraph) and graph.requires_grad:
         token, slot = graph.new_slot(z.size(1))
         return _Aggregate.apply(z, token, graph, slot)
@@ -497,6 +507,7 @@ def keyed_dropout(x: torch.Tensor, p: float, key, residual: Optional[torch.Tenso
     result is rounded once.  key: (seed, tag, counter), see
     ldsgnn.rng.Generator.dropout_key; p in [0, 1]."""
     keep, scale = _keep_scale(p, key, "dropout")
+    _no_tangent("dropout", x, residual)
     _element_code(x, "dropout")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or
                                  residual.device != x.device):
@@ -668,6 +679,7 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] 
     code = ACTIVATIONS.get(act)
     if code is None:
         raise ValueError(f"ldsgnn group_norm_act: unknown activation {act!r}; one of {sorted(ACTIVATIONS)}")
+    _no_tangent("group_norm_act", x, weight, bias)
     _element_code(x, "group_norm_act")
     if x.dim() < 2:
         raise ValueError(f"ldsgnn group_norm_act: expected (..., n, C), got {tuple(x.shape)}")
@@ -745,6 +757,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     even (lds_quantize_rows).  A zero row gives q = 0, scale = 0; a row with an
     infinity or a NaN gives scale NaN.  For weights (out × in) the same call
     gives a scale per output channel.  No gradient."""
+    _no_tangent("quantize_rows", x)
     code = _element_code(x, "quantize_rows")
     if x.dim() != 2:
         raise ValueError(f"ldsgnn quantize_rows: expected rows × k, got {tuple(x.shape)}")
@@ -758,6 +771,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 
 def _no_grad_only(what: str, *tensors) -> None:
+    _no_tangent(what, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"ldsgnn {what}: the 8-bit product has no gradient; call it under torch.no_grad()")
 

@@ -42,6 +42,27 @@ def test_no_gradient_through_the_8_bit_product():
         ops.int8_matmul(q, torch.ones(4), q, torch.ones(4), bias=torch.zeros(4, requires_grad=True))
 
 
+@pytest.mark.parametrize("which", ["x", "residual", "norm x", "weight", "bias", "quantize", "matmul scale", "linear x",
+                                   "linear bias", "aggregate"])
+def test_tangents_are_refused(which):
+    """A forward-mode derivative is not computed, so it is not dropped in silence
+    either: the refusal comes before any other check."""
+    from torch.autograd import forward_ad
+    x, c = torch.randn(4, 8), torch.ones(8)
+    q, one = torch.zeros(4, 16, dtype=torch.int8), torch.ones(4)
+    calls = {"x": lambda d: ops.keyed_dropout(d(x), 0.5, KEY), "residual": lambda d: ops.keyed_dropout(x, 0.5, KEY, d(x)),
+             "norm x": lambda d: ops.group_norm_act(d(x), 2), "weight": lambda d: ops.group_norm_act(x, 2, d(c)),
+             "bias": lambda d: ops.group_norm_act(x, 2, c, d(c)), "quantize": lambda d: ops.quantize_rows(d(x)),
+             "matmul scale": lambda d: ops.int8_matmul(q, d(one), q, one), "linear x": lambda d: ops.int8_linear(d(x), q, one),
+             "linear bias": lambda d: ops.int8_linear(x, q, one, d(one)), "aggregate": lambda d: ops.aggregate(d(x), None)}
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            calls[which](lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises((RuntimeError, AttributeError)) as other:  # no tangent: the next check (no device here)
+            calls[which](lambda t: t)
+        assert not isinstance(other.value, NotImplementedError)
+
+
 def _drop(**kw):
     a = dict(x=FAKE, ldx=8, res=0, ldr=0, y=FAKE, ldy=8, rows=4, cols=8, dtype=0, keep=0.5, scale=2.0)
     a.update(kw)
