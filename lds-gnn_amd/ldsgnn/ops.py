@@ -650,6 +650,8 @@ class _GroupNormActGrad(Function):
         pl, need = ctx.pl, ctx.need
         inputs = [None if t is None else t.detach().requires_grad_(True) for t in ctx.saved_tensors]
         gy, x, weight, bias = inputs
+        if x.numel() == 0:  # the first order is zeros, whatever the inputs
+            return tuple(None if t is None else torch.zeros_like(t) for t in inputs) + (None, None, None)
         mask = None
         if pl.keep < 1.0:
             mask = _dropout_raw(torch.ones(x.shape, dtype=torch.float32, device=x.device), pl.mask)

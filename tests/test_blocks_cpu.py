@@ -42,6 +42,25 @@ def test_no_gradient_through_the_8_bit_product():
         ops.int8_matmul(q, torch.ones(4), q, torch.ones(4), bias=torch.zeros(4, requires_grad=True))
 
 
+def check_empty_second_order(norm, shape, groups, device):
+    """The second derivative of an empty tensor: zeros, as the first order gives."""
+    leaves = [torch.randn(s, device=device, requires_grad=True) for s in (shape, shape[-1:], shape[-1:])]
+    dy = torch.randn(shape, device=device, requires_grad=True)
+    y = norm(*leaves)
+    first = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    total = sum((f * torch.ones_like(f)).sum() for f in first)
+    for t, g in zip([dy] + leaves, torch.autograd.grad(total, [dy] + leaves)):
+        assert g.shape == t.shape and not g.any()
+
+
+@pytest.mark.parametrize("shape,groups", [((0, 3, 4), 2), ((2, 0, 4), 2), ((2, 3, 0), 1), ((0, 4), 4), ((0, 0, 0), 3)])
+@pytest.mark.parametrize("act,p", [("none", 0.0), ("silu", 0.5), ("relu", 1.0)])
+def test_second_order_of_an_empty_norm(shape, groups, act, p):
+    keep = 1.0 - p
+    pl = ops._NormPlan(groups, ops.ACTIVATIONS[act], 1e-5, keep, 1.0 / keep if keep else 0.0, KEY)
+    check_empty_second_order(lambda x, w, b: ops._GroupNormAct.apply(x, w, b, pl), shape, groups, "cpu")
+
+
 @pytest.mark.parametrize("which", ["x", "residual", "norm x", "weight", "bias", "quantize", "matmul scale", "linear x",
                                    "linear bias", "aggregate"])
 def test_tangents_are_refused(which):

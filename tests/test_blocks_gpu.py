@@ -578,6 +578,13 @@ def test_group_norm_empty(device, ops, shape):
     assert y.shape == x.shape and x.grad.shape == x.shape and float(w.grad.sum()) == 0.0
 
 
+@pytest.mark.parametrize("shape,groups", [((0, 3, 4), 2), ((2, 0, 4), 2), ((2, 3, 0), 1), ((0, 4), 4)])
+def test_group_norm_second_order_of_an_empty_tensor(device, ops, shape, groups):
+    from tests.test_blocks_cpu import check_empty_second_order
+    check_empty_second_order(lambda x, w, b: ops.group_norm_act(x, groups, w, b, act="silu", p=0.5, key=KEY), shape,
+                             groups, device)
+
+
 @pytest.mark.parametrize("weight,bias", [(True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("pdtype", DTYPES)
 def test_group_norm_parameter_forms(device, ops, weight, bias, pdtype):
