@@ -258,7 +258,7 @@ def chain_us(fn, dev, k, reps=3):
     s.wait_stream(torch.cuda.current_stream(dev))
     g = torch.cuda.CUDAGraph()
     with torch.cuda.stream(s):
-        with torch.cuda.graph(g, stream=s):
+        with nat.no_collection(), torch.cuda.graph(g, stream=s):
             for _ in range(k):
                 fn(nat.stream_of(dev))
         g.replay()
@@ -333,7 +333,7 @@ def window_breakdown(eng, reducer, args, device, k=20, reps=10, rounds=5):
         st = torch.cuda.Stream(device=device)
         st.wait_stream(cur)
         with torch.cuda.stream(st):
-            with torch.cuda.graph(g, stream=st):
+            with nat.no_collection(), torch.cuda.graph(g, stream=st):
                 restore()
                 for name, a, _ in calls[:j]:
                     real(name, *(a[:-1] + (nat.stream_of(device),)))

@@ -8,8 +8,11 @@ is missing, importing ldsgnn raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import gc
 import os
+import threading
 
 import torch  # noqa: F401  (must precede the CDLL: shared HIP runtime)
 
@@ -280,6 +283,32 @@ UPLOAD_GRAPHS = True
 # collective), the event nodes a collective library may add to order its own
 # stream against the capture
 _GRAPH_NODE_OK_EXCHANGE = {**_GRAPH_NODE_OK, 6: "event wait", 7: "event record"}
+
+
+_collection_lock = threading.Lock()
+_collection_off = [0, False]  # captures inside no_collection(), whether the first of them found collection on
+
+
+@contextlib.contextmanager
+def no_collection():
+    """No garbage collection inside, in any thread: a collected CUDAGraph (an
+    engine's, in a reference cycle) synchronizes the device as it goes, which a
+    capture does not permit, and its destructor ends the process over that.
+    Every capture in the package runs inside; one of a caller's own belongs
+    inside too.  Captures of several threads may overlap: collection is back on
+    when the last of them is done."""
+    with _collection_lock:
+        if _collection_off[0] == 0:
+            _collection_off[1] = gc.isenabled()
+            gc.disable()
+        _collection_off[0] += 1
+    try:
+        yield
+    finally:
+        with _collection_lock:
+            _collection_off[0] -= 1
+            if _collection_off[0] == 0 and _collection_off[1]:
+                gc.enable()
 
 
 def graph_census(graph: "torch.cuda.CUDAGraph") -> dict:

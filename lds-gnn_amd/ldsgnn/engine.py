@@ -35,9 +35,7 @@ S = 1 is the reference's single chain.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-import gc
 from collections import OrderedDict
 from typing import List, Optional
 
@@ -133,20 +131,6 @@ def _csr_of(dense: torch.Tensor):
             sp.values().to(torch.float32).contiguous())
 
 
-@contextlib.contextmanager
-def _no_collection():
-    """No garbage collection inside: a collected CUDAGraph (an engine's, in a
-    reference cycle) synchronizes the device as it goes, which a capture does
-    not permit, and its destructor ends the process over that."""
-    on = gc.isenabled()
-    gc.disable()
-    try:
-        yield
-    finally:
-        if on:
-            gc.enable()
-
-
 def capture_into(graph, stream, body, pool=None, error_mode: str = "global", joins=()):
     """Capture body() into `graph` on `stream` (torch.cuda.CUDAGraph
     capture_begin / capture_end).
@@ -159,7 +143,7 @@ def capture_into(graph, stream, body, pool=None, error_mode: str = "global", joi
     error is re-raised.  Without this, torch.cuda.graph's __exit__ raised
     hipErrorStreamCaptureUnjoined on top of the real cause (
     "What's weak" #8) and left the stream capturing."""
-    with _no_collection(), torch.cuda.stream(stream):
+    with nat.no_collection(), torch.cuda.stream(stream):
         if pool is None:
             graph.capture_begin(capture_error_mode=error_mode)
         else:
@@ -1741,7 +1725,7 @@ class LdsEngine:
             tail.capture_begin(pool=pool)
 
         err = None
-        with _no_collection(), torch.cuda.stream(s):
+        with nat.no_collection(), torch.cuda.stream(s):
             head.capture_begin(pool=pool)
             try:
                 self.run_window(tau, grad_reducer=switch)

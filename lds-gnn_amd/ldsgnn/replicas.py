@@ -20,6 +20,8 @@ from typing import Optional
 import torch
 import torch.distributed as dist
 
+from . import _native as nat
+
 
 def _group_up() -> bool:
     return dist.is_available() and dist.is_initialized()
@@ -101,7 +103,7 @@ def collective_capture_probe(device: torch.device) -> bool:
         s = torch.cuda.Stream(device)
         s.wait_stream(torch.cuda.current_stream(device))
         with torch.cuda.stream(s):
-            with torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
+            with nat.no_collection(), torch.cuda.graph(graph, stream=s, capture_error_mode="thread_local"):
                 dist.all_reduce(x, op=dist.ReduceOp.SUM)
         torch.cuda.current_stream(device).wait_stream(s)
     except Exception:  # noqa: BLE001  (any capture failure means: do not capture)

@@ -142,6 +142,82 @@ def test_no_garbage_collection_inside_a_capture(fake_cuda, fails):
         gc.enable()
 
 
+def test_overlapping_captures_keep_collection_off():
+    """Two threads capture at once: the first to finish does not turn collection
+    back on under the other."""
+    import gc
+    import threading
+    a_in, b_in, a_out = (threading.Event() for _ in range(3))
+    seen = []
+
+    def first():
+        with nat.no_collection():
+            a_in.set()
+            assert b_in.wait(30)
+        a_out.set()
+
+    def second():
+        assert a_in.wait(30)
+        with nat.no_collection():
+            b_in.set()
+            assert a_out.wait(30)
+            seen.append(gc.isenabled())
+
+    assert gc.isenabled()
+    threads = [threading.Thread(target=f) for f in (first, second)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert seen == [False] and gc.isenabled()
+    with nat.no_collection():  # one inside another
+        with nat.no_collection():
+            pass
+        assert not gc.isenabled()
+    assert gc.isenabled()
+
+
+@pytest.mark.parametrize("fails", [False, True])
+def test_no_garbage_collection_inside_the_captured_collective(monkeypatch, fails):
+    """The probe that captures an all-reduce holds collection off for the capture."""
+    import gc
+
+    from ldsgnn import replicas
+    seen = []
+
+    class Graph:
+        def replay(self):
+            pass
+
+    class Stream:
+        def wait_stream(self, other):
+            pass
+
+    @contextlib.contextmanager
+    def capture(graph, stream=None, capture_error_mode=None):
+        seen.append(("begin", gc.isenabled()))
+        yield
+        seen.append(("end", gc.isenabled()))
+
+    def all_reduce(t, op=None):
+        if t.dtype == torch.float32:
+            seen.append(("collective", gc.isenabled()))
+            if fails:
+                raise RuntimeError("cannot be captured")
+
+    monkeypatch.setattr(replicas, "_group_up", lambda: True)
+    monkeypatch.setattr(replicas, "exchange_capturable", lambda: True)
+    monkeypatch.setattr(replicas.dist, "get_world_size", lambda: 1)
+    monkeypatch.setattr(replicas.dist, "all_reduce", all_reduce)
+    for name, fake in (("CUDAGraph", Graph), ("Stream", lambda d: Stream()), ("current_stream", lambda d: Stream()),
+                       ("stream", lambda s: contextlib.nullcontext()), ("graph", capture),
+                       ("synchronize", lambda d: None)):
+        monkeypatch.setattr(torch.cuda, name, fake)
+    assert replicas.collective_capture_probe(torch.device("cpu")) is (not fails)
+    assert [on for _, on in seen] == [False] * len(seen) and len(seen) == (2 if fails else 3)
+    assert gc.isenabled()
+
+
 def test_capture_status_classes():
     assert E._capture_status(None) == E._CAPTURE_OK
     assert E._capture_status(nat.NativeError("x")) == E._CAPTURE_FATAL

@@ -21,11 +21,12 @@ import torch  # noqa: E402
 
 
 def graph_time(fn, reps=5):
+    from ldsgnn import _native as nat
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     g = torch.cuda.CUDAGraph()
     with torch.cuda.stream(s):
-        with torch.cuda.graph(g, stream=s):
+        with nat.no_collection(), torch.cuda.graph(g, stream=s):
             fn()
     torch.cuda.current_stream().wait_stream(s)
     g.replay()
