@@ -13,7 +13,11 @@ from ..trainers import Metrics
 
 def _int8_form(model, params):
     from ..models.gcn import Int8DenseGCN
-    return model if isinstance(model, Int8DenseGCN) else Int8DenseGCN(model, params)
+    if not isinstance(model, Int8DenseGCN):
+        return Int8DenseGCN(model, params)
+    if params is not None:
+        raise ValueError("Int8DenseGCN holds its own weights: quantise new ones with Int8DenseGCN(model, params)")
+    return model
 
 
 def accuracy(predictions: torch.Tensor, labels: torch.Tensor) -> float:

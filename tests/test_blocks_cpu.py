@@ -82,6 +82,18 @@ def test_tangents_are_refused(which):
         assert not isinstance(other.value, NotImplementedError)
 
 
+def test_8_bit_evaluation_does_not_ignore_weights():
+    """empirical_mean_loss with weights for a model that already holds its own."""
+    from collections import OrderedDict
+
+    from ldsgnn.models.gcn import Int8DenseGCN
+    from ldsgnn.utils.evaluation import empirical_mean_loss
+    model = Int8DenseGCN.__new__(Int8DenseGCN)
+    torch.nn.Module.__init__(model)
+    with pytest.raises(ValueError, match="own weights"):
+        empirical_mean_loss(model, torch.nn.Module(), 0, None, model_parameters=OrderedDict(), int8=True)
+
+
 def _drop(**kw):
     a = dict(x=FAKE, ldx=8, res=0, ldr=0, y=FAKE, ldy=8, rows=4, cols=8, dtype=0, keep=0.5, scale=2.0)
     a.update(kw)
