@@ -147,10 +147,8 @@ def prepare(case, seed):
     if own:
         st["ops"] = _ops()
         if case["op"] == "int8":
-            # the weights laid out once; quantised activations as quantize_rows lays them out
+            # the weights laid out once; activations are new at every call, which lays them out itself
             st["wq"] = st["ops"].int8_rows(st["wq"])
-            if not case["dynamic"]:
-                st["xq"] = st["ops"].int8_rows(st["xq"])
         elif case["train"]:
             for name in ("x", "w", "b", "res"):
                 if name in st:
