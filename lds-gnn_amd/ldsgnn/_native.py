@@ -361,7 +361,10 @@ def ptr(t) -> int:
 
 
 def stream_of(device) -> int:
-    """The current stream of a device (torch.device or index) as a hipStream_t."""
+    """The current stream of a device (torch.device, index, name, or None: the
+    current one) as a hipStream_t."""
+    if not isinstance(device, (int, torch.device)):
+        device = torch.device("cuda" if device is None else device)
     index = device if isinstance(device, int) else device.index
     # the handle itself (0.1 us on the host); current_stream() builds a Stream object (2 us)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)

@@ -913,6 +913,14 @@ def _block_inputs(ops, device):
     return x, w, b, dy, wq, ws
 
 
+def test_stream_of_takes_what_names_a_device(device):
+    from ldsgnn import _native as nat
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for name in (device, 0, "cuda", "cuda:0", None, torch.device("cuda")):
+            assert nat.stream_of(name) == side.cuda_stream, name
+
+
 def test_side_stream_runs_the_same_bits(device, ops):
     args = _block_inputs(ops, device)
     ref = _all_ops(ops, *args)
