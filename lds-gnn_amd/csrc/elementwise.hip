@@ -20,7 +20,7 @@ namespace lds {
 // No lane branches before its loads, so all of them are in flight at once; with
 // the last vector element by element instead, 40000 x 512 of fp16 took 28 us and
 // x 511 74, now 22 and 22.  Bound by memory: 160000 x 512 bf16 with a residual
-// 75 us (6.5 TB/s), 20000 x 257 fp16 9.1, 2708 x 1433 fp32 6.4.
+// 75 us (6.6 TB/s), 20000 x 257 fp16 8.2, 2708 x 1433 fp32 6.3.
 template <typename T, int V, bool RES, bool DROP, bool PAST>
 __global__ __launch_bounds__(256) void dropout_add_kernel(const T* x, int64_t ldx, const T* res, int64_t ldr,
                                                           T* y, int64_t ldy, int64_t rows, int cols, int cvecs,

@@ -112,7 +112,7 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 
 // The V values of a row from j < cols on, zeros behind its end: one whole load that
 // ends with the row at most, moved down by what lies before j.  cols >= V.  (Element
-// by element, 20000 rows of 4095 bf16 took 71 us to quantise, so 49; of 4096 47.)
+// by element, 20000 rows of 4095 bf16 took 71 us to quantise, so 44; of 4096 alike.)
 template <typename T, int V>
 __device__ __forceinline__ void load_to_end(const T* __restrict__ row, int j, int cols, float (&f)[V]) {
     static_assert(V * sizeof(T) == 16, "two 64-bit halves");
@@ -135,8 +135,8 @@ __device__ __forceinline__ void load_to_end(const T* __restrict__ row, int j, in
     for (int e = 0; e < V; ++e) f[e] = elem<T, V>(u.raw, e);
 }
 
-// Bound by memory where rows are long (20000 x 4096 bf16: 42.5 us, 5.8 TB/s), by the
-// waves' latency where they are short (20000 x 128: 4.3 us).
+// Bound by memory where rows are long (20000 x 4096 bf16: 43 to 50 us by the clock,
+// 5.7 to 4.9 TB/s), by the waves' latency where they are short (20000 x 128: 4.6 us).
 // G lanes per row (a power of two up to the block), R vectors of V values a lane
 // held in registers between the two uses of a row; a row longer than G R V is
 // read again.  The largest |x| is found on the bits, so that an infinity or a
@@ -243,7 +243,7 @@ __device__ __forceinline__ void put_y(const Int8Args& a, T* __restrict__ y, int6
 
 // A 16 MF x 16 NF tile of y per block; its W waves take W slices of k, four steps of
 // 64 bytes in flight, and meet in LDS.  For few rows, where the weights' bytes
-// are the bound: 1 x 4096 x 4096 4.2 us (4.0 TB/s), 64 rows 7.9 us.
+// are the bound: 1 x 4096 x 4096 4.5 us (3.7 TB/s), 64 rows 8.4 us.
 template <typename T, int MF, int NF, int W>
 __global__ __launch_bounds__(64 * W) void int8_split_kernel(Int8Args a, T* __restrict__ y) {
     constexpr int kAhead = 4;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * W) void int8_split_kernel(Int8Args a, T* __res
 // One or two rows (single nodes): every block quantises the rows into LDS by
 // itself, under the loads of its first weights, and multiplies them with 16
 // rows of w, k split over its eight waves.  One launch: 1 x 4096 x 4096 from
-// bf16 5.4 us, against 7.7 for quantiser and product.  With a slower rounding
+// bf16 5.8 us, against 7.9 for quantiser and product.  With a slower rounding
 // two rows took 8.1 / 8.4 us and four 10.9 / 8.5, so it ends at two.
 constexpr int kFewRows = 2, kFewBytes = 32768;
 template <typename TX, int V>
@@ -433,9 +433,9 @@ __device__ const v4i kZeroChunk = {0, 0, 0, 0};
 // row r sits at place c ^ (r / 4 % 4), so that the 16 lanes of a read phase, one
 // chunk of 16 rows, meet 16 different 16-byte bank groups (no conflict counted).
 //
-// 8192^3: 500 us, 2200 TOP/s (the library's int8 product of that size on the same
-// card: 544 us); 20000 x 4096 x 4096: 340 us, 1970 TOP/s.  Bound by power: with zeros
-// in x and w the latter takes 250 us, at random values the clock is 1.8 GHz and
+// 8192^3: 520 us, 2115 TOP/s (the library's int8 product of that size: 544 us);
+// 20000 x 4096 x 4096: 331 us, 2030 TOP/s.  Bound by power: with zeros
+// in x and w the latter takes 240 us, at random values the clock is 1.8 GHz and
 // the matrix units are busy 54 % of its cycles.
 template <typename T, int BM, int BN, int WM, int WN, int kStages>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(Int8Args a, T* __restrict__ y) {

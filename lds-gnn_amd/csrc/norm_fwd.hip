@@ -31,7 +31,7 @@ __device__ __forceinline__ void apply_quad(const Quad<T, V>& x, const QuadRows& 
 // ---------------------------------------------------------------------------
 // slab: one block, a sample's rows of a few groups, Q quads a thread.  Bound by
 // its chain of latencies (one load, two block sums, one store): one node of 32
-// groups of 8, bf16, 4.7 us; 2708 x 4 groups of 4, fp32 with dropout, 8.8.
+// groups of 8, bf16, 4.6 us; 2708 x 4 groups of 4, fp32 with dropout, 8.7.
 // ---------------------------------------------------------------------------
 
 template <typename T, int V, int ACT, bool DROP, int Q>
@@ -112,8 +112,8 @@ __global__ __launch_bounds__(1024) void gn_slab_kernel(const T* x, NormArgs a, f
 }
 
 // ---------------------------------------------------------------------------
-// parts.  Bound by memory: 8 x 20000 x 256 bf16 (82 MB) statistics 17.5 us, result
-// 27.5 (x comes from the memory-side cache the second time); with dropout 36,
+// parts.  Bound by memory: 8 x 20000 x 256 bf16 (82 MB) statistics 17.3 us, result
+// 27.0 (x comes from the memory-side cache the second time); with dropout 34,
 // bound by the vector units (24 operations a value, half of them the mask).
 // ---------------------------------------------------------------------------
 
